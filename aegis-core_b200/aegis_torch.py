@@ -1,4 +1,6 @@
-"""torch.ops.aegis.matmul: the library's GEMM as a PyTorch operator.
+"""torch.ops.aegis: the library's operators as PyTorch operators.
+
+matmul: the 16-bit GEMM.
 
     import aegis_torch  # registers the op
     C = torch.ops.aegis.matmul(A, B)      # A [M, K], B [K, N], both f16 or both bf16, on one CUDA device
@@ -13,6 +15,22 @@ A fake implementation gives shapes under meta and fake tensors.
 
 It is the Python-side counterpart of the reference's C++ aegis::matmul and
 only plumbing: the GEMM is the same C-ABI call every other caller makes.
+
+The 8-bit operators (include/aegis_i8.h has their definitions; sm_100 only):
+
+    q, s    = torch.ops.aegis.rmsnorm_i8(x, weight, eps)                # x [M, K] f16 or bf16
+    q, s, h = torch.ops.aegis.add_rmsnorm_i8(x, residual, weight, eps)  # h = x + residual
+    y       = torch.ops.aegis.matmul_i8(q, w, s, w_scale, bias=None, out_dtype=torch.bfloat16)  # w [N, K] int8
+    q, s    = torch.ops.aegis.silu_mul_i8(gate, up)
+    y, h    = torch.ops.aegis.mlp_i8(x, residual, norm_weight, eps, w_gate_up, s_gate_up, w_down, s_down)
+
+They run on torch's current stream of their operands' device, may be captured
+into CUDA graphs after one call on the device, and have fake implementations.
+Rows may be strided (stride(-1) == 1, rows that do not overlap); other stride
+patterns are copied first. The int8 results have rows padded to 16 bytes
+(stride(0) is a multiple of 16), which is what the product reads fastest.
+They have no backward pass: an input that requires a gradient is refused
+while gradients are recorded.
 """
 from __future__ import annotations
 
@@ -22,6 +40,7 @@ import torch
 from torch.library import custom_op
 
 import aegis_capi as ac
+import aegis_i8 as i8
 
 _lock = threading.Lock()
 _contexts: dict[int, ac.Context] = {}
@@ -80,3 +99,259 @@ def _(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
     torch._check(a.dim() == 2 and b.dim() == 2, lambda: "aegis::matmul takes 2-D operands")
     torch._check(a.shape[1] == b.shape[0], lambda: "aegis::matmul: inner sizes differ")
     return a.new_empty((a.shape[0], b.shape[1]))
+
+
+# ---------------------------------------------------------------- 8-bit operators
+_DTYPE_CODE = {torch.float16: i8.DTYPE_F16, torch.bfloat16: i8.DTYPE_BF16, torch.float32: i8.DTYPE_F32}
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+_defs = torch.library.Library("aegis", "FRAGMENT")
+_defs.define("matmul_i8(Tensor a, Tensor w, Tensor a_scale, Tensor w_scale, Tensor? bias=None, *, "
+             "ScalarType? out_dtype=None) -> Tensor")
+_defs.define("rmsnorm_i8(Tensor x, Tensor weight, float eps) -> (Tensor, Tensor)")
+_defs.define("add_rmsnorm_i8(Tensor x, Tensor residual, Tensor weight, float eps) -> (Tensor, Tensor, Tensor)")
+_defs.define("silu_mul_i8(Tensor gate, Tensor up) -> (Tensor, Tensor)")
+_defs.define("mlp_i8(Tensor x, Tensor residual, Tensor norm_weight, float eps, Tensor w_gate_up, Tensor s_gate_up, "
+             "Tensor w_down, Tensor s_down) -> (Tensor, Tensor)")
+
+
+def _rows(t: torch.Tensor):
+    """(tensor, row stride) of a 2-D operand whose rows are contiguous and do not overlap, else of a copy."""
+    st0, st1 = t.stride()
+    rows, cols = t.shape
+    if (st1 == 1 or cols <= 1) and (st0 >= cols or rows <= 1):
+        # A single row has no stride of its own: one that every kernel can take.
+        return t, (st0 if rows > 1 else (cols + 15) // 16 * 16)
+    t = t.contiguous()
+    return t, max(cols, 1)
+
+
+def _vector(t: torch.Tensor) -> torch.Tensor:
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _no_grad(name: str, *tensors) -> None:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"aegis::{name} has no backward pass: call it under torch.no_grad() or detach "
+                                   "its inputs")
+
+
+def _same_device(name: str, first: torch.Tensor, *others) -> None:
+    d = first.device
+    for t in others:
+        if t is not None and t.device != d:
+            raise ValueError(f"aegis::{name}: operands on different devices ({d} and {t.device})")
+
+
+def _f32_vector(name: str, what: str, t: torch.Tensor, n) -> None:
+    if t.dtype != torch.float32:
+        raise TypeError(f"aegis::{name}: {what} must be float32, not {t.dtype}")
+    if t.dim() != 1 or t.shape[0] != n:
+        raise ValueError(f"aegis::{name}: {what} must have shape ({n},), not {tuple(t.shape)}")
+
+
+def _check_matmul_i8(a, w, a_scale, w_scale, bias, out_dtype):
+    name = "matmul_i8"
+    if a.dim() != 2 or w.dim() != 2:
+        raise ValueError("aegis::matmul_i8 takes 2-D operands")
+    if a.dtype != torch.int8 or w.dtype != torch.int8:
+        raise TypeError(f"aegis::matmul_i8: a and w must be int8, not {a.dtype} and {w.dtype}")
+    if a.shape[1] != w.shape[1]:
+        raise ValueError(f"aegis::matmul_i8: a [M, K] and w [N, K] have different K ({tuple(a.shape)}, {tuple(w.shape)})")
+    if a.shape[1] > i8.MAX_K:
+        raise ValueError(f"aegis::matmul_i8: K above {i8.MAX_K}: the int32 sum could overflow")
+    _f32_vector(name, "a_scale", a_scale, a.shape[0])
+    _f32_vector(name, "w_scale", w_scale, w.shape[0])
+    if out_dtype is None:
+        out_dtype = bias.dtype if bias is not None else torch.bfloat16
+    if out_dtype not in _DTYPE_CODE:
+        raise TypeError(f"aegis::matmul_i8: out_dtype must be float16, bfloat16 or float32, not {out_dtype}")
+    if bias is not None:
+        if bias.dtype != out_dtype:
+            raise TypeError(f"aegis::matmul_i8: bias must have the output's type, {out_dtype}")
+        if bias.dim() != 1 or bias.shape[0] != w.shape[0]:
+            raise ValueError(f"aegis::matmul_i8: bias must have shape ({w.shape[0]},), not {tuple(bias.shape)}")
+    _same_device(name, a, w, a_scale, w_scale, bias)
+    _no_grad(name, a_scale, w_scale, bias)
+    return out_dtype
+
+
+def _matmul_i8(a, w, a_scale, w_scale, bias=None, *, out_dtype=None):
+    out_dtype = _check_matmul_i8(a, w, a_scale, w_scale, bias, out_dtype)
+    M, K = a.shape
+    N = w.shape[0]
+    dev = a.get_device()
+    out = torch.empty((M, N), dtype=out_dtype, device=a.device)
+    if M and N:
+        a, lda = _rows(a)
+        w, ldw = _rows(w)
+        a_scale, w_scale = _vector(a_scale), _vector(w_scale)
+        if bias is not None:
+            bias = _vector(bias)
+        st = i8.load().aegis_i8_gemm(dev, _raw_stream(dev), _DTYPE_CODE[out_dtype], M, N, K, a.data_ptr(), lda,
+                                     w.data_ptr(), ldw, a_scale.data_ptr(), w_scale.data_ptr(),
+                                     None if bias is None else bias.data_ptr(), out.data_ptr(), N)
+        if st:
+            i8.check(st, "aegis::matmul_i8")
+    return out
+
+
+def _matmul_i8_meta(a, w, a_scale, w_scale, bias=None, *, out_dtype=None):
+    out_dtype = _check_matmul_i8(a, w, a_scale, w_scale, bias, out_dtype)
+    return a.new_empty((a.shape[0], w.shape[0]), dtype=out_dtype)
+
+
+def _empty_codes(x: torch.Tensor):
+    """(q, scale) for the rows of x: int8 rows 16 bytes aligned, one float a row."""
+    rows, cols = x.shape
+    return (torch.empty_strided((rows, cols), ((cols + 15) // 16 * 16, 1), dtype=torch.int8, device=x.device),
+            torch.empty((rows,), dtype=torch.float32, device=x.device))
+
+
+def _check_rows(name, x, y, what):
+    if x.dim() != 2:
+        raise ValueError(f"aegis::{name} takes 2-D operands")
+    if x.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"aegis::{name}: operands must be float16 or bfloat16, not {x.dtype}")
+    if x.shape[1] == 0:
+        raise ValueError(f"aegis::{name}: rows of no elements have no scale")
+    if y is not None:
+        if y.dtype != x.dtype:
+            raise TypeError(f"aegis::{name}: {what} must have x's type, {x.dtype}, not {y.dtype}")
+        if y.shape != x.shape:
+            raise ValueError(f"aegis::{name}: {what} must have shape {tuple(x.shape)}, not {tuple(y.shape)}")
+
+
+def _check_norm(name, x, residual, weight, eps):
+    _check_rows(name, x, residual, "residual")
+    if weight.dtype != x.dtype:
+        raise TypeError(f"aegis::{name}: weight must have x's type, {x.dtype}, not {weight.dtype}")
+    if weight.dim() != 1 or weight.shape[0] != x.shape[1]:
+        raise ValueError(f"aegis::{name}: weight must have shape ({x.shape[1]},), not {tuple(weight.shape)}")
+    if not 0.0 <= eps <= 3.4e38:
+        raise ValueError(f"aegis::{name}: eps must be a finite number, 0 or more")
+    _same_device(name, x, residual, weight)
+    _no_grad(name, x, residual, weight)
+
+
+def _norm(name, x, residual, weight, eps):
+    _check_norm(name, x, residual, weight, eps)
+    q, scale = _empty_codes(x)
+    h = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    rows, cols = x.shape
+    if rows:
+        dev = x.get_device()
+        x, ldx = _rows(x)
+        r, ldr = (None, 0) if residual is None else _rows(residual)
+        weight = _vector(weight)
+        st = i8.load().aegis_i8_rmsnorm(dev, _raw_stream(dev), _DTYPE_CODE[x.dtype], rows, cols, x.data_ptr(), ldx,
+                                        None if r is None else r.data_ptr(), ldr, weight.data_ptr(), eps,
+                                        None if h is None else h.data_ptr(), cols, q.data_ptr(), q.stride(0),
+                                        scale.data_ptr())
+        if st:
+            i8.check(st, f"aegis::{name}")
+    return q, scale, h
+
+
+def _rmsnorm_i8(x, weight, eps):
+    return _norm("rmsnorm_i8", x, None, weight, eps)[:2]
+
+
+def _rmsnorm_i8_meta(x, weight, eps):
+    _check_norm("rmsnorm_i8", x, None, weight, eps)
+    return _empty_codes(x)
+
+
+def _add_rmsnorm_i8(x, residual, weight, eps):
+    return _norm("add_rmsnorm_i8", x, residual, weight, eps)
+
+
+def _add_rmsnorm_i8_meta(x, residual, weight, eps):
+    _check_norm("add_rmsnorm_i8", x, residual, weight, eps)
+    return (*_empty_codes(x), x.new_empty(x.shape))
+
+
+def _check_silu_mul(gate, up):
+    _check_rows("silu_mul_i8", gate, up, "up")
+    _same_device("silu_mul_i8", gate, up)
+    _no_grad("silu_mul_i8", gate, up)
+
+
+def _silu_mul_i8(gate, up):
+    _check_silu_mul(gate, up)
+    q, scale = _empty_codes(gate)
+    rows, cols = gate.shape
+    if rows:
+        dev = gate.get_device()
+        gate, ldg = _rows(gate)
+        up, ldu = _rows(up)
+        st = i8.load().aegis_i8_silu_mul(dev, _raw_stream(dev), _DTYPE_CODE[gate.dtype], rows, cols, gate.data_ptr(),
+                                         ldg, up.data_ptr(), ldu, q.data_ptr(), q.stride(0), scale.data_ptr())
+        if st:
+            i8.check(st, "aegis::silu_mul_i8")
+    return q, scale
+
+
+def _silu_mul_i8_meta(gate, up):
+    _check_silu_mul(gate, up)
+    return _empty_codes(gate)
+
+
+def _check_mlp(x, residual, norm_weight, eps, w_gate_up, s_gate_up, w_down, s_down):
+    name = "mlp_i8"
+    _check_norm(name, x, residual, norm_weight, eps)
+    for what, w in (("w_gate_up", w_gate_up), ("w_down", w_down)):
+        if w.dtype != torch.int8:
+            raise TypeError(f"aegis::mlp_i8: {what} must be int8, not {w.dtype}")
+        if w.dim() != 2:
+            raise ValueError(f"aegis::mlp_i8: {what} must have two dimensions")
+    K, F = x.shape[1], w_down.shape[1]
+    if w_gate_up.shape != (2 * F, K) or w_down.shape[0] != K:
+        raise ValueError(f"aegis::mlp_i8: x [M, K], w_gate_up [2F, K] and w_down [K, F] do not fit "
+                         f"({tuple(x.shape)}, {tuple(w_gate_up.shape)}, {tuple(w_down.shape)})")
+    if F == 0 or F > i8.MAX_K or K > i8.MAX_K:
+        raise ValueError(f"aegis::mlp_i8: K and F must be from 1 to {i8.MAX_K}")
+    _f32_vector(name, "s_gate_up", s_gate_up, 2 * F)
+    _f32_vector(name, "s_down", s_down, K)
+    _same_device(name, x, w_gate_up, s_gate_up, w_down, s_down)
+    _no_grad(name, s_gate_up, s_down)
+
+
+def _mlp_i8(x, residual, norm_weight, eps, w_gate_up, s_gate_up, w_down, s_down):
+    _check_mlp(x, residual, norm_weight, eps, w_gate_up, s_gate_up, w_down, s_down)
+    M, K = x.shape
+    F = w_down.shape[1]
+    y = torch.empty((M, K), dtype=x.dtype, device=x.device)
+    h = torch.empty((M, K), dtype=x.dtype, device=x.device)
+    if M:
+        dev = x.get_device()
+        x, ldx = _rows(x)
+        r, ldr = _rows(residual)
+        w1, ld1 = _rows(w_gate_up)
+        w2, ld2 = _rows(w_down)
+        g, s1, s2 = _vector(norm_weight), _vector(s_gate_up), _vector(s_down)
+        nbytes = i8.mlp_workspace(M, K, F)
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=x.device)  # torch's allocator: 512-byte aligned
+        st = i8.load().aegis_i8_mlp(dev, _raw_stream(dev), _DTYPE_CODE[x.dtype], M, K, F, x.data_ptr(), ldx,
+                                    r.data_ptr(), ldr, g.data_ptr(), eps, w1.data_ptr(), ld1, s1.data_ptr(),
+                                    w2.data_ptr(), ld2, s2.data_ptr(), h.data_ptr(), K, y.data_ptr(), K,
+                                    ws.data_ptr(), nbytes)
+        if st:
+            i8.check(st, "aegis::mlp_i8")
+    return y, h
+
+
+def _mlp_i8_meta(x, residual, norm_weight, eps, w_gate_up, s_gate_up, w_down, s_down):
+    _check_mlp(x, residual, norm_weight, eps, w_gate_up, s_gate_up, w_down, s_down)
+    return x.new_empty(x.shape), x.new_empty(x.shape)
+
+
+for _name, _cuda, _meta in (("matmul_i8", _matmul_i8, _matmul_i8_meta),
+                            ("rmsnorm_i8", _rmsnorm_i8, _rmsnorm_i8_meta),
+                            ("add_rmsnorm_i8", _add_rmsnorm_i8, _add_rmsnorm_i8_meta),
+                            ("silu_mul_i8", _silu_mul_i8, _silu_mul_i8_meta),
+                            ("mlp_i8", _mlp_i8, _mlp_i8_meta)):
+    _defs.impl(_name, _cuda, "CUDA")
+    _defs.impl(_name, _meta, "Meta")

@@ -1,0 +1,61 @@
+#pragma once
+// Internal host interface of the 8-bit operators (include/aegis_i8.h has the
+// definitions). Every function launches on the current device.
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace aegis::i8 {
+
+enum class Out : int { F16 = 0, BF16 = 1, F32 = 2 };
+
+struct Gemm {
+  const void* A = nullptr;  // M x K int8
+  const void* W = nullptr;  // N x K int8
+  const float* a_scale = nullptr;
+  const float* w_scale = nullptr;
+  const void* bias = nullptr;
+  void* C = nullptr;
+  int M = 0, N = 0, K = 0;
+  long long lda = 0, ldw = 0, ldc = 0;
+  Out out = Out::BF16;
+  // The kernel launched just before on this stream is one of this file's row
+  // operations, which let their dependents start only after everything before
+  // them has completed: the weights may then be read before that kernel ends.
+  bool weights_settled = false;
+};
+
+// Which kernel runs, and how the work is cut.
+struct GemmPlan {
+  bool pair = false;  // CTA pairs on 256 x 256 tiles; else the stream kernel
+  int tile_m = 0;     // tokens a tile
+  int tile_n = 0;     // channels a tile
+  int splits = 1;     // slices of K, one CTA of a cluster each (stream kernel)
+  long long tiles = 0, grid = 0;
+};
+GemmPlan plan_gemm(int M, int N, int K, bool tma, int sms);
+
+// Whether TMA can address the rows: 16-byte aligned base, stride a multiple of 16.
+bool tma_rows(const void* p, long long ld);
+
+cudaError_t gemm(const Gemm& g, cudaStream_t s);
+
+struct RowOp {
+  bool bf16 = false;
+  int rows = 0, cols = 0;
+  const void* x = nullptr;         // or gate
+  long long ldx = 0;
+  const void* residual = nullptr;  // or up
+  long long ldr = 0;
+  const void* weight = nullptr;
+  float eps = 0.f;
+  void* h = nullptr;
+  long long ldh = 0;
+  void* q = nullptr;
+  long long ldq = 0;
+  float* scale = nullptr;
+};
+cudaError_t rmsnorm(const RowOp& r, cudaStream_t s);
+cudaError_t silu_mul(const RowOp& r, cudaStream_t s);
+
+}  // namespace aegis::i8

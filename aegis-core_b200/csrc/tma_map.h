@@ -1,5 +1,5 @@
 #pragma once
-// TMA tensor-map encoding for 16-bit operands (cuTensorMapEncodeTiled through
+// TMA tensor-map encoding for 16-bit and 8-bit operands (cuTensorMapEncodeTiled through
 // the runtime's driver entry point, so the library needs no libcuda link).
 #include <cuda.h>
 
@@ -12,5 +12,9 @@ namespace aegis {
 // coordinate is unused. False if the driver refuses the geometry.
 bool encode_map(CUtensorMap* map, gemm::DType dt, const void* base, long long inner, long long outer, long long ld,
                 long long batch, long long bstride, int box_outer);
+
+// The same for rows of 8-bit codes: boxes of {128, box_outer, 1}, ld in bytes
+// (a multiple of 16, as is the base address).
+bool encode_map_i8(CUtensorMap* map, const void* base, long long inner, long long outer, long long ld, int box_outer);
 
 }  // namespace aegis
