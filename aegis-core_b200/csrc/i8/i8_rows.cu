@@ -6,17 +6,26 @@
 // whole row and drops out of q; it enters the scale alone, m / rms / 127. For the
 // norm t = h * weight is a product of two 16-bit numbers, exact in float; so q
 // is a definite whole number, and both operations give exactly the nearest one
-// (of t in 64 bits): the quotient is taken in float, whose error is below
-// kBand, and the few elements that come nearer than that to the border between
-// two codes are computed again in double. Codes therefore do not depend on a
-// row's layout, its neighbours or the number of threads.
+// (of t in 64 bits): z = 127 t / m is taken in float, with a bound on its error,
+// and the few elements that come nearer than that to the border between two
+// codes are computed again in double. Codes therefore do not depend on a row's
+// layout, its neighbours or the number of threads.
 //
-// Bound: memory. One block holds one row in registers (up to 32 elements a
-// thread), reads it once and writes it once; rows beyond 32768 elements take
-// two passes, the second one out of L2.
+// Bound: memory for the norm, instruction issue and memory alike for silu (about
+// 25 instructions an element). The blocks that fit the GPU walk the rows, a thread
+// with up to 32 elements, so what a row costs besides its elements (reduction,
+// barrier) is spread over many. A thread copies its elements of the next row to
+// shared memory while it works on this one, and reads them itself, so the copies
+// need no barrier and no row's loads wait for the reduction of the one before. t
+// stays in registers between the maximum and the codes. One barrier a row: silu's
+// elements at a border need the maximum in 64 bits, which its holder works out
+// meanwhile; they are set right after the next row's barrier. Few rows take more threads
+// with fewer elements each, for latency. Rows beyond 32768 elements, and rows
+// that do not start on 16-byte boundaries, are read directly.
 #include <algorithm>
 
 #include "../common.cuh"
+#include "../gpu_target.h"
 #include "../ptx.cuh"
 #include "i8.h"
 
@@ -26,7 +35,7 @@ namespace {
 enum Mode : int { kNorm = 0, kAddNorm = 1, kSilu = 2 };
 
 struct RowArgs {
-  int cols;
+  int rows, cols;
   const void* x;  // or gate
   long long ldx;
   const void* r;  // residual, or up
@@ -42,16 +51,28 @@ struct RowArgs {
   int vec_q;  // every row of q starts on an 8-byte boundary
 };
 
-// |127 t / m| in float is off by less than this. Norm: t and m are exact, the
-// factor 127 / m and the product round once each: 127 * 2 * 2^-24 = 1.5e-5.
-// Silu: t and m carry the errors of expf (2 ulp), the sum, the quotient and
-// the product, below 5 * 2^-24 * 1.5 each: 127 * 17 * 2^-24 = 1.3e-4.
-template <int MODE>
-constexpr float kBand = MODE == kSilu ? 2.5e-4f : 3e-5f;
-// How far below the float maximum the true one can lie, relative: both carry the error above.
-constexpr float kNearMax = 1.f - 4e-6f;
-// Row maxima below this leave float's range of full precision: the row is done in double.
-constexpr float kTiny = 1e-30f;
+// The error of z = t * (127 / m) in float, relative, with u = 2^-24.
+// Norm: t and m are exact; the factor and the product round once each: 2 u.
+// Silu, t = x / (1 + e) * y with e = 2^(-x log2 e): the power's argument is off by
+// 1.25 u |x| log2 e, the power by that and by 4 u; the sum u, the reciprocal 2 u,
+// two products 2 u; then the factor (m and the quotient rounded) 2 u and the last
+// product u: (1.25 |x| + 12) u, the first part for negative x alone.
+// The factor may come from the float maximum, off by (1.25 |x| + 9) u itself.
+constexpr float kBorderNorm = 1.5e-7f;
+__device__ __forceinline__ float border_silu(float gate) { return fmaf(gate, 1.6e-7f, 1.4e-6f); }
+// How far below the float maximum the true one can lie, relative.
+__device__ __forceinline__ float near_max(float gate) { return 1.f - fmaf(gate, 1.5e-7f, 1.25e-6f); }
+// What that error bound needs: e far from overflow, and no product near the
+// end of float's range. Rows with other values are done in double.
+constexpr float kMostGate = 80.f, kMostUp = 1e15f;  // gates below 0 alone
+// Rows whose largest magnitude is below this are done in double: float's range ends near.
+constexpr float kTiny = 1e-20f;
+constexpr double kMost = 3.4028234663852886e38;  // the largest float
+// Adding this rounds a float below 2^22 to a whole number (nearest, ties to
+// even) and leaves that number's two's complement in the low bits, without
+// the conversion unit, which the exponential and the reciprocal need.
+constexpr float kRound = 12582912.f;  // 1.5 * 2^23
+constexpr float kNearBorder = 0.4999999f;
 
 // 8 elements from column c on (those beyond cols: 0).
 template <class T>
@@ -74,25 +95,57 @@ __device__ __forceinline__ void store8(T* row, int c, int cols, bool vec, uint4 
   for (int i = 0; i < 8; ++i)
     if (c + i < cols) reinterpret_cast<uint16_t*>(row)[c + i] = uint16_t(u[i >> 1] >> (16 * (i & 1)));
 }
-template <class T>
-__device__ __forceinline__ void unpack8(uint4 v, float (&f)[8]) {
-  const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 p = Elem<T>::pair_to_f32(u[i]);
-    f[2 * i] = p.x;
-    f[2 * i + 1] = p.y;
-  }
+// Two floats in a register pair: sm_100 adds, multiplies and fuses both at once.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pair(float a, float b) {
+  f32x2 d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
 }
-__device__ __forceinline__ void store_codes(int8_t* row, int c, int cols, bool vec, const int (&q)[8]) {
-  const uint32_t lo = (q[0] & 255) | (q[1] & 255) << 8 | (q[2] & 255) << 16 | uint32_t(q[3] & 255) << 24;
-  const uint32_t hi = (q[4] & 255) | (q[5] & 255) << 8 | (q[6] & 255) << 16 | uint32_t(q[7] & 255) << 24;
+__device__ __forceinline__ float2 both(f32x2 v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+// The largest magnitude of three, a NaN if one is.
+__device__ __forceinline__ float max_abs_nan(float a, float2 b) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b.x), "f"(b.y));
+  return d;
+}
+template <class T>
+__device__ __forceinline__ f32x2 widen(uint32_t v) {
+  const float2 f = Elem<T>::pair_to_f32(v);
+  return pair(f.x, f.y);
+}
+template <class T>
+__device__ __forceinline__ uint32_t narrow(f32x2 v) {
+  const float2 f = both(v);
+  return Elem<T>::pack(f.x, f.y);
+}
+// 8 codes to columns c.. of a row.
+__device__ __forceinline__ void store_codes(int8_t* row, int c, int cols, bool vec, uint2 q) {
   if (vec && c + 8 <= cols) {
-    *reinterpret_cast<uint2*>(row + c) = make_uint2(lo, hi);
+    *reinterpret_cast<uint2*>(row + c) = q;
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (c + i < cols) row[c + i] = int8_t(q[i]);
+      if (c + i < cols) row[c + i] = int8_t((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
   }
 }
 
@@ -121,210 +174,559 @@ struct Row {
   }
 };
 
+// 2^x, off by at most 2^-22, relative.
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 1 / x, off by at most 2^-23, for x from 1 to 2^126.
+__device__ __forceinline__ float fast_reciprocal(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// x * sigmoid(x) * y.
+__device__ __forceinline__ f32x2 silu_mul(f32x2 x, f32x2 y) {
+  const float2 p = both(mul2(x, pair(-1.44269504f, -1.44269504f)));
+  const float2 d = both(add2(pair(fast_exp2(p.x), fast_exp2(p.y)), pair(1.f, 1.f)));
+  return mul2(mul2(x, pair(fast_reciprocal(d.x), fast_reciprocal(d.y))), y);
+}
+
+template <class T> struct Pair;
+template <> struct Pair<__half> { using type = __half2; };
+template <> struct Pair<__nv_bfloat16> { using type = __nv_bfloat162; };
+
+// What a thread gathers of its elements in a row.
+template <class T>
+struct Stats {
+  using P = typename Pair<T>::type;
+  float m = 0.f;   // max |t|
+  f32x2 ss = 0;    // squares, of even and odd elements (norm)
+  uint32_t low = 0, high = 0;  // least gate, largest |up|, two at a time (silu)
+  __device__ void gate_up(uint32_t g, uint32_t u) {
+    const P l = __hmin2(reinterpret_cast<const P&>(low), reinterpret_cast<const P&>(g));
+    const P h = __hmax2(reinterpret_cast<const P&>(high), __habs2(reinterpret_cast<const P&>(u)));
+    low = reinterpret_cast<const uint32_t&>(l);
+    high = reinterpret_cast<const uint32_t&>(h);
+  }
+  __device__ float gate() const {  // magnitude of the least gate below 0
+    const float2 f = Elem<T>::pair_to_f32(low);
+    return -fminf(f.x, f.y);
+  }
+  __device__ float most_up() const {
+    const float2 f = Elem<T>::pair_to_f32(high);
+    return fmaxf(f.x, f.y);
+  }
+};
+
+// t of 8 elements, given the packed inputs; returns what is normalised (h, or x).
 template <class T, int MODE>
-__device__ __forceinline__ void eval8(const RowArgs& a, const Row<T, MODE>& row, int c, float (&t)[8], float& ss) {
-  float x[8], y[8];
-  unpack8<T>(load8(row.x, c, a.cols, a.vec), x);
-  if constexpr (MODE == kSilu) {
-    unpack8<T>(load8(row.r, c, a.cols, a.vec), y);
+__device__ __forceinline__ uint4 eval8(uint4 xv, uint4 yv, uint4 wv, f32x2 (&t)[4], Stats<T>& st) {
+  uint32_t x[4] = {xv.x, xv.y, xv.z, xv.w};
+  const uint32_t y[4] = {yv.x, yv.y, yv.z, yv.w}, w[4] = {wv.x, wv.y, wv.z, wv.w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = x[i] / (1.f + expf(-x[i])) * y[i];
-    // expf(-x) overflows below -88: the quotient is then -0, as it should be
-    // in float (kTiny covers rows where that is all there is).
-  } else {
-    if constexpr (MODE == kAddNorm) {
-      unpack8<T>(load8(row.r, c, a.cols, a.vec), y);
-      uint4 hv;
-      hv.x = Elem<T>::pack(x[0] + y[0], x[1] + y[1]);
-      hv.y = Elem<T>::pack(x[2] + y[2], x[3] + y[3]);
-      hv.z = Elem<T>::pack(x[4] + y[4], x[5] + y[5]);
-      hv.w = Elem<T>::pack(x[6] + y[6], x[7] + y[7]);
-      store8(row.h, c, a.cols, a.vec, hv);
-      unpack8<T>(hv, x);
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (MODE == kAddNorm) x[i] = narrow<T>(add2(widen<T>(x[i]), widen<T>(y[i])));
+    const f32x2 f = widen<T>(x[i]);
+    if constexpr (MODE == kSilu) {
+      t[i] = silu_mul(f, widen<T>(y[i]));
+      st.gate_up(x[i], y[i]);
+    } else {
+      t[i] = mul2(f, widen<T>(w[i]));
+      st.ss = fma2(f, f, st.ss);
     }
-    unpack8<T>(load8(row.w, c, a.cols, a.vec), y);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      t[i] = x[i] * y[i];
-      ss = fmaf(x[i], x[i], ss);
-    }
+    st.m = max_abs_nan(st.m, both(t[i]));
   }
+  return make_uint4(x[0], x[1], x[2], x[3]);
+}
+// The same from memory, columns c.. of a row; stores h.
+template <class T, int MODE>
+__device__ __forceinline__ void load_eval8(const RowArgs& a, const Row<T, MODE>& row, int c, f32x2 (&t)[4],
+                                           Stats<T>& st) {
+  const uint4 none = make_uint4(0, 0, 0, 0);
+  const uint4 h = eval8<T, MODE>(load8(row.x, c, a.cols, a.vec),
+                                 MODE == kNorm ? none : load8(row.r, c, a.cols, a.vec),
+                                 MODE == kSilu ? none : load8(row.w, c, a.cols, a.vec), t, st);
+  if constexpr (MODE == kAddNorm) store8(row.h, c, a.cols, a.vec, h);
 }
 
+// A block's results: max |t|, the sum of the squares, the magnitude of the least
+// gate. Magnitudes are compared as the bits of floats without a sign, where a NaN
+// is above infinity.
+struct Found {
+  float m, ss, gate;
+};
+__device__ __forceinline__ float max_bits(float v) {
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
+}
+template <int MODE>
+__device__ __forceinline__ Found block_find(float m, float ss, float gate, int* any, Found* buf) {
+  const int W = int(blockDim.x) / 32;
+  const int lane = int(threadIdx.x & 31);
+  Found f;
+  f.m = max_bits(fabsf(m));
+  f.gate = MODE == kSilu ? max_bits(fabsf(gate)) : 0.f;
+  if (MODE != kSilu)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  f.ss = ss;
+  if (lane == 0) buf[threadIdx.x >> 5] = f;
+  if (MODE == kSilu) *any = __syncthreads_or(*any);
+  else __syncthreads();
+  if (W > 1) {
+    f = lane < W ? buf[lane] : Found{0.f, 0.f, 0.f};
+    f.m = max_bits(f.m);
+    if (MODE == kSilu) {
+      f.gate = max_bits(f.gate);
+    } else {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) f.ss += __shfl_xor_sync(0xffffffffu, f.ss, o);
+    }
+  }
+  return f;
+}
 // max that keeps a NaN.
-__device__ __forceinline__ float max_nan(float a, float b) { return a > b || a != a ? a : b; }
+__device__ __forceinline__ double max_nan(double a, double b) { return a > b || a != a ? a : b; }
 
-// Every thread of the block gets the block's results; `buf` may be used again after the next barrier.
-template <int THREADS>
-__device__ __forceinline__ float2 block_max_sum(float m, float s, float2* buf) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-    s += __shfl_xor_sync(0xffffffffu, s, o);
-  }
-  constexpr int W = THREADS / 32;
-  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = make_float2(m, s);
-  __syncthreads();
-  float2 v = buf[0];
-#pragma unroll
-  for (int i = 1; i < W; ++i) {
-    v.x = max_nan(v.x, buf[i].x);
-    v.y += buf[i].y;
-  }
-  return v;
-}
-template <int THREADS>
-__device__ __forceinline__ double block_reduce64(double v, bool sum, double* buf) {
-#pragma unroll
+// The block's sum or maximum in double. Out of line: rare rows only.
+__device__ __noinline__ double block_reduce64(double v, bool sum, double* buf) {
   for (int o = 16; o > 0; o >>= 1) {
     const double u = __shfl_xor_sync(0xffffffffu, v, o);
-    v = sum ? v + u : fmax(v, u);
+    v = sum ? v + u : max_nan(v, u);
   }
   __syncthreads();
   if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
   __syncthreads();
   v = buf[0];
-  for (int i = 1; i < THREADS / 32; ++i) v = sum ? v + buf[i] : fmax(v, buf[i]);
+  for (int i = 1; i < int(blockDim.x) / 32; ++i) v = sum ? v + buf[i] : max_nan(v, buf[i]);
   return v;
 }
 
-// VPT pieces of 8 elements a thread in registers; VPT = 0: rows of any length, two passes.
-template <class T, int MODE, int THREADS, int VPT>
-__global__ void __launch_bounds__(THREADS) i8_row_kernel(const __grid_constant__ RowArgs a) {
-  __shared__ float2 buf[THREADS / 32];
-  __shared__ double buf64[THREADS / 32];
+// The code of column c in 64 bits. Out of line: one copy for the few elements at a border.
+template <class T, int MODE>
+__device__ __noinline__ int code64(Row<T, MODE> row, int c, double m64) {
+  return int(rint(127.0 * row.t64(c) / m64));
+}
+template <class T, int MODE>
+__device__ __noinline__ double abs_t64(Row<T, MODE> row, int c) {
+  return fabs(row.t64(c));
+}
+
+// The sum of the row's squares in double, for rows whose squares leave float's range.
+template <class T, int MODE>
+__device__ __noinline__ double squares64(Row<T, MODE> row, int cols, double* buf) {
+  double s = 0.0;
+  for (int c0 = int(threadIdx.x) * 8; c0 < cols; c0 += int(blockDim.x) * 8)
+    for (int c = c0; c < min(c0 + 8, cols); ++c) s += row.norm_input(c) * row.norm_input(c);
+  return block_reduce64(s, true, buf);
+}
+
+// A row of zeros, or of numbers for which float's range or precision does not
+// do, all in double. Each thread reads the columns whose h it stored itself.
+// Returns the row's maximum.
+template <class T, int MODE>
+__device__ __noinline__ double row_in_double(Row<T, MODE> row, int cols, int8_t* q, double* buf) {
+  double m = 0.0;
+  for (int c0 = int(threadIdx.x) * 8; c0 < cols; c0 += int(blockDim.x) * 8)
+    for (int c = c0; c < min(c0 + 8, cols); ++c) m = max_nan(fabs(row.t64(c)), m);
+  m = block_reduce64(m, false, buf);
+  for (int c0 = int(threadIdx.x) * 8; c0 < cols; c0 += int(blockDim.x) * 8)
+    for (int c = c0; c < min(c0 + 8, cols); ++c) q[c] = m > 0.0 && m <= kMost ? int8_t(code64<T, MODE>(row, c, m)) : int8_t(0);
+  return m;
+}
+
+__device__ __forceinline__ float at(const f32x2 (&t)[4], int i) {
+  const float2 f = both(t[i >> 1]);
+  return i & 1 ? f.y : f.x;
+}
+
+// 8 codes n from t. An element nearer to a border than z's error, border |z|, has
+// to be taken again: with d the distance from z to n, d > 1/2 - border (|n| + 1/2).
+// `most` gathers a first test of all elements, (most > first_test(border)) if
+// there may be one: border (n^2 / 64 + 16) for border |n|, which is never less, and
+// d^2 for d, to spare the magnitudes.
+__device__ __forceinline__ uint2 quantise8(const f32x2 (&t)[4], float inv, float border, float& most) {
+  uint32_t code[8];
+  const f32x2 inv2 = pair(inv, inv), up = pair(kRound, kRound);
+  const f32x2 minus = pair(-1.f, -1.f), b2 = pair(border / 64.f, border / 64.f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const f32x2 r = fma2(t[i], inv2, up), n = fma2(r, minus, up);  // -n
+    const f32x2 d = fma2(t[i], inv2, n);
+    most = max_abs_nan(most, both(fma2(mul2(n, b2), n, mul2(d, d))));
+    const float2 f = both(r);
+    code[2 * i] = __float_as_uint(f.x);
+    code[2 * i + 1] = __float_as_uint(f.y);
+  }
+  const uint32_t a = __byte_perm(code[0], code[1], 0x0040), b = __byte_perm(code[2], code[3], 0x0040);
+  const uint32_t d = __byte_perm(code[4], code[5], 0x0040), e = __byte_perm(code[6], code[7], 0x0040);
+  return make_uint2(__byte_perm(a, b, 0x5410), __byte_perm(d, e, 0x5410));
+}
+__device__ __forceinline__ float first_test(float border) { return 0.2499998f - 16.5f * border; }
+// A bit for each of the 8 elements that is nearer to a border than that.
+__device__ __forceinline__ uint32_t near_border(const f32x2 (&t)[4], float inv, float border) {
+  uint32_t near = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float n = __fsub_rn(fmaf(at(t, i), inv, kRound), kRound);
+    near |= fmaf(fabsf(n) + 0.5f, border, fabsf(fmaf(at(t, i), inv, -n))) > kNearBorder ? 1u << i : 0u;
+  }
+  return near;
+}
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// What the two kernels below share: the row's maximum in 64 bits, its scale, and what
+// silu leaves to do until the next row's barrier.
+template <class T, int MODE>
+struct Finish {
+  const RowArgs& a;
+  unsigned long long* top64;  // row maxima in 64 bits, of three rows in turn: the bits
+                              // of a double that is not negative order as it does
+  double* buf64;
+  uint32_t border_bits = 0;   // elements of row `behind` at a border (silu)
+  int behind = -1;
+  unsigned slot = 0;          // its place in top64
+  unsigned turn = 0;          // this row's: 0, 1, 2, 0, ...
+  double m64 = 0.0;
+
+  __device__ int column(int i) const {  // of the thread's i-th element
+    return ((i >> 3) * int(blockDim.x) + int(threadIdx.x)) * 8 + (i & 7);
+  }
+  __device__ void set_codes(int ri, uint32_t bits, double top) const {
+    const Row<T, MODE> row(a, ri);
+    for (; bits; bits &= bits - 1) {
+      const int c = column(__ffs(int(bits)) - 1);
+      if (c < a.cols) a.q[(long long)ri * a.ldq + c] = int8_t(code64<T, MODE>(row, c, top));
+    }
+  }
+  // Silu, between the barriers of the next row and the one after it (or behind
+  // a barrier of its own). Where it is called, t is no longer needed: t kept over the
+  // calls in here cost 34 registers' spills a row.
+  __device__ void settle() {
+    if (MODE != kSilu || behind < 0) return;
+    const double top = __longlong_as_double((long long)top64[slot]);
+    if (threadIdx.x == 0) a.scale[behind] = float(top / 127.0);
+    if (border_bits) set_codes(behind, border_bits, top);
+    border_bits = 0;
+    behind = -1;
+  }
+  // Right after row ri's barrier. True: the row is done (not finite, or in double).
+  __device__ bool begin(int ri, const Found& f, int in_double) {
+    if (MODE == kSilu && threadIdx.x == 0) top64[turn == 2 ? 0 : turn + 1] = 0;  // the next row's; its readers are past the barrier
+    in_double |= f.m < kTiny;
+    m64 = double(f.m);
+    if (!in_double && f.m <= 3.4028235e38f) return false;
+    const Row<T, MODE> row(a, ri);
+    int8_t* q = a.q + (long long)ri * a.ldq;
+    if (in_double) m64 = row_in_double<T, MODE>(row, a.cols, q, buf64);
+    if (!(m64 <= kMost)) {
+      // Not finite: codes 0, scale NaN. (An infinite h gives a t that is infinite, or NaN where the weight is 0.)
+      for (int c0 = int(threadIdx.x) * 8; c0 < a.cols; c0 += int(blockDim.x) * 8)
+        for (int c = c0; c < min(c0 + 8, a.cols); ++c) q[c] = 0;
+      if (threadIdx.x == 0) a.scale[ri] = __int_as_float(0x7fc00000);
+    } else if (MODE == kSilu) {
+      if (threadIdx.x == 0) a.scale[ri] = float(m64 / 127.0);
+    } else {
+      norm_scale(ri, f);
+    }
+    return true;
+  }
+  __device__ void norm_scale(int ri, const Found& f) const {
+    if (!(f.ss < 1e37f) || f.ss < 1e-25f) {  // squares that left float's range are summed again in double
+      const double sum = squares64<T, MODE>(Row<T, MODE>(a, ri), a.cols, buf64);
+      if (threadIdx.x == 0)
+        a.scale[ri] = m64 > 0.0 ? float(m64 / (127.0 * sqrt(sum / a.cols + double(a.eps)))) : 0.f;
+    } else if (threadIdx.x == 0) {
+      a.scale[ri] = float(m64) / (127.f * sqrtf(f.ss / float(a.cols) + a.eps));
+    }
+  }
+  // Silu: element i of this thread can be the row's maximum.
+  __device__ void candidate(int ri, int i) const {
+    const double d = abs_t64<T, MODE>(Row<T, MODE>(a, ri), column(i));
+    atomicMax(&top64[turn], (unsigned long long)__double_as_longlong(d));
+  }
+  // The end of row ri: settles the row before, and leaves `bits` of this one for later (done: nothing).
+  __device__ void end(int ri, uint32_t bits, bool done) {
+    settle();
+    if (!done) {
+      border_bits = bits;
+      behind = ri;
+      slot = turn;
+    }
+    turn = turn == 2 ? 0 : turn + 1;
+  }
+};
+
+// Many rows. Blocks of as many threads as a row of 32 elements a thread takes;
+// every row starts on a 16-byte boundary (q's on 8) and has whole pieces.
+constexpr int kPieces = 4;
+template <class T, int MODE, int MOST, int BLOCKS>
+__global__ void __launch_bounds__(MOST, BLOCKS) i8_rows_kernel(const __grid_constant__ RowArgs a) {
+  extern __shared__ uint4 ahead[];  // the next row: [piece][source][thread]
+  __shared__ Found buf[2][32];
+  __shared__ double buf64[32];
+  __shared__ unsigned long long top64[3];
+  constexpr int kSources = MODE == kNorm ? 1 : 2;
+  const int tid = int(threadIdx.x), step = int(blockDim.x) * 8, c0 = tid * 8;
+  if (tid < 3) top64[tid] = 0;
   // Programmatic dependent launch: nothing is read before the grids this one
   // depends on have completed. The kernels after this one may start once every
   // block has come this far, so what came before it has completed for them too.
   ptx::griddep_wait();
   ptx::griddep_launch_dependents();
-  const Row<T, MODE> row(a, blockIdx.x);
-  int8_t* q = a.q + (long long)blockIdx.x * a.ldq;
-  float t[VPT ? VPT : 1][8];
-  float m = 0.f, ss = 0.f;
-  if constexpr (VPT > 0) {
-#pragma unroll
-    for (int v = 0; v < VPT; ++v) {
-      const int c = (v * THREADS + int(threadIdx.x)) * 8;
-      if (c < a.cols) {
-        eval8<T, MODE>(a, row, c, t[v], ss);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) m = max_nan(fabsf(t[v][i]), m);
-      }
-    }
-  } else {
-    for (int c = int(threadIdx.x) * 8; c < a.cols; c += THREADS * 8) {
-      eval8<T, MODE>(a, row, c, t[0], ss);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) m = max_nan(fabsf(t[0][i]), m);
-    }
-  }
-  const float2 red = block_max_sum<THREADS>(m, ss, buf);
-  m = red.x;
-  ss = red.y;
 
-  // Not finite: codes 0, scale NaN. (A finite t from an h that is not: inf * 0 is NaN, so t shows it.)
-  if (!(m <= 3.4028235e38f)) {
-    const int zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    for (int c = int(threadIdx.x) * 8; c < a.cols; c += THREADS * 8) store_codes(q, c, a.cols, a.vec_q, zero);
-    if (threadIdx.x == 0) a.scale[blockIdx.x] = __int_as_float(0x7fc00000);
-    return;
-  }
-  // The row's maximum in 64 bits: that of the elements which can be it.
-  const bool slow = m < kTiny;  // every element in double
-  double m64 = double(m);
-  if (MODE == kSilu || slow) {
-    double mine = 0.0;
-    if (slow) {
-      for (int c = int(threadIdx.x) * 8; c < a.cols; c += THREADS * 8)
-        for (int i = 0; i < 8 && c + i < a.cols; ++i) mine = fmax(mine, fabs(row.t64(c + i)));
-    } else {
-      const float near = m * kNearMax;
-#pragma unroll(VPT ? VPT : 1)
-      for (int v = 0; v < (VPT ? VPT : 1 << 30); ++v) {
-        const int c = (v * THREADS + int(threadIdx.x)) * 8;
-        if (c >= a.cols) break;
-        float tt[8], unused = 0.f;
-        if constexpr (VPT == 0) eval8<T, MODE>(a, row, c, tt, unused);
+  const int pieces = c0 < a.cols ? min(kPieces, (a.cols - 1 - c0) / step + 1) : 0;
+  const int rows_ahead = int(gridDim.x);
+  const T* x = static_cast<const T*>(a.x) + (long long)blockIdx.x * a.ldx + c0;
+  const T* r = MODE == kNorm ? nullptr : static_cast<const T*>(a.r) + (long long)blockIdx.x * a.ldr + c0;
+  const T* w = MODE == kSilu ? nullptr : static_cast<const T*>(a.w) + c0;
+  T* h = MODE == kAddNorm ? static_cast<T*>(a.h) + (long long)blockIdx.x * a.ldh + c0 : nullptr;
+  int8_t* q = a.q + (long long)blockIdx.x * a.ldq + c0;
+  const uint32_t mine = ptx::smem_addr(ahead) + uint32_t(tid) * 16u, source = blockDim.x * 16u;
+  auto copy_piece = [&](int v) {
+    copy16(mine + uint32_t(v * kSources) * source, x + v * step);
+    if (MODE != kNorm) copy16(mine + uint32_t(v * kSources + 1) * source, r + v * step);
+  };
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (fabsf(VPT ? t[VPT ? v : 0][i] : tt[i]) >= near && c + i < a.cols) mine = fmax(mine, fabs(row.t64(c + i)));
+  for (int v = 0; v < kPieces; ++v)
+    if (v < pieces) copy_piece(v);
+  copy_commit();
+
+  Finish<T, MODE> fin{a, top64, buf64};
+  unsigned par = 0;
+  for (int ri = int(blockIdx.x);; par ^= 1u) {
+    const bool more = a.rows - ri > rows_ahead;
+    x += (long long)rows_ahead * a.ldx;
+    if (MODE != kNorm) r += (long long)rows_ahead * a.ldr;
+    f32x2 t[kPieces][4];
+    Stats<T> st;
+    copy_wait<0>();
+#pragma unroll
+    for (int v = 0; v < kPieces; ++v) {
+      if (v < pieces) {
+        const uint4 xv = ptx::ld_shared_v4(mine + uint32_t(v * kSources) * source);
+        const uint4 yv = MODE == kNorm ? xv : ptx::ld_shared_v4(mine + uint32_t(v * kSources + 1) * source);
+        const uint4 hv = eval8<T, MODE>(xv, yv, MODE == kSilu ? xv : *reinterpret_cast<const uint4*>(w + v * step),
+                                        t[v], st);
+        if (MODE == kAddNorm) *reinterpret_cast<uint4*>(h + v * step) = hv;
+        if (more) copy_piece(v);
       }
     }
-    m64 = block_reduce64<THREADS>(mine, false, buf64);
+    copy_commit();
+    const int in_double = MODE == kSilu && (st.gate() > kMostGate || (Elem<T>::kBf16 && st.most_up() > kMostUp));
+    int any = in_double;
+    const Found f = block_find<MODE>(st.m, both(st.ss).x + both(st.ss).y, st.gate(), &any, buf[par]);
+    const bool done = fin.begin(ri, f, any);
+    uint32_t near = 0, can = 0;
+    if (!done) {
+      const float inv = 127.f / f.m;
+      const float border = MODE == kSilu ? border_silu(f.gate) : kBorderNorm;
+      float most = 0.f;
+#pragma unroll
+      for (int v = 0; v < kPieces; ++v)
+        if (v < pieces) *reinterpret_cast<uint2*>(q + v * step) = quantise8(t[v], inv, border, most);
+      if (most > first_test(border)) {
+#pragma unroll
+        for (int v = 0; v < kPieces; ++v)
+          if (v < pieces) near |= near_border(t[v], inv, border) << (8 * v);
+      }
+      // The maximum in 64 bits is that of the elements which can be it.
+      const float least = f.m * near_max(f.gate);
+      if (MODE == kSilu && st.m >= least) {
+#pragma unroll
+        for (int v = 0; v < kPieces; ++v)
+          if (v < pieces)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) can |= fabsf(at(t[v], i)) >= least ? 1u << (8 * v + i) : 0u;
+      }
+      if (MODE != kSilu) fin.norm_scale(ri, f);
+    }
+    if constexpr (MODE == kSilu) {
+      for (; can; can &= can - 1) fin.candidate(ri, __ffs(int(can)) - 1);
+      fin.end(ri, near, done);
+    } else if (near) {
+      fin.set_codes(ri, near, fin.m64);
+    }
+    if (!more) break;
+    ri += rows_ahead;
+    q += (long long)rows_ahead * a.ldq;
+    if (MODE == kAddNorm) h += (long long)rows_ahead * a.ldh;
   }
   if constexpr (MODE == kSilu) {
-    if (threadIdx.x == 0) a.scale[blockIdx.x] = float(m64 / 127.0);
-  } else {
-    // Squares that left float's range are summed again in double.
-    double sum = double(ss);
-    if (!(ss < 1e37f) || ss < 1e-25f) {
-      double s64 = 0.0;
-      for (int c = int(threadIdx.x) * 8; c < a.cols; c += THREADS * 8)
-        for (int i = 0; i < 8 && c + i < a.cols; ++i) s64 += row.norm_input(c + i) * row.norm_input(c + i);
-      sum = block_reduce64<THREADS>(s64, true, buf64);
-    }
-    if (threadIdx.x == 0)
-      a.scale[blockIdx.x] = m64 > 0.0 ? float(m64 / (127.0 * sqrt(sum / a.cols + double(a.eps)))) : 0.f;
+    __syncthreads();
+    fin.settle();
   }
+}
 
-  const float inv = slow ? 0.f : 127.f / float(m64);
-#pragma unroll(VPT ? VPT : 1)
-  for (int v = 0; v < (VPT ? VPT : 1 << 30); ++v) {
-    const int c = (v * THREADS + int(threadIdx.x)) * 8;
-    if (c >= a.cols) break;
-    float tt[8], unused = 0.f;
-    if constexpr (VPT == 0) {
+// Any rows, one a block: few rows, rows of any alignment, and with VPT = 0 of any
+// length (VPT pieces of 8 elements a thread; 0: as many as it takes, read twice).
+template <class T, int MODE, int THREADS, int VPT>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) i8_row_kernel(const __grid_constant__ RowArgs a) {
+  __shared__ Found buf[32];
+  __shared__ double buf64[32];
+  __shared__ unsigned long long top64[3];
+  constexpr int kKept = VPT ? VPT : 1;
+  const int tid = int(threadIdx.x), ri = int(blockIdx.x);
+  auto piece = [&](int v) { return (v * THREADS + tid) * 8; };
+  if (tid < 3) top64[tid] = 0;
+  ptx::griddep_wait();  // as above
+  ptx::griddep_launch_dependents();
+  const Row<T, MODE> row(a, ri);
+  int8_t* q = a.q + (long long)ri * a.ldq;
+  f32x2 t[kKept][4];
+  Stats<T> st;
+  if constexpr (VPT > 0) {
+#pragma unroll
+    for (int v = 0; v < VPT; ++v)
+      if (piece(v) < a.cols) load_eval8<T, MODE>(a, row, piece(v), t[v], st);
+  } else {
+    for (int v = 0; piece(v) < a.cols; ++v) load_eval8<T, MODE>(a, row, piece(v), t[0], st);
+  }
+  int any = MODE == kSilu && (st.gate() > kMostGate || st.most_up() > kMostUp);
+  const Found f = block_find<MODE>(st.m, both(st.ss).x + both(st.ss).y, st.gate(), &any, buf);
+  Finish<T, MODE> fin{a, top64, buf64};
+  if (fin.begin(ri, f, any)) return;
+  const float inv = 127.f / f.m;
+  const float border = MODE == kSilu ? border_silu(f.gate) : kBorderNorm;
+  const float least = f.m * near_max(f.gate);
+  if constexpr (VPT > 0) {
+    float most = 0.f;
+    uint32_t near = 0;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v)
+      if (piece(v) < a.cols)
+        store_codes(q, piece(v), a.cols, a.vec_q, quantise8(t[v], inv, border, most));
+    if (most > first_test(border)) {
+#pragma unroll
+      for (int v = 0; v < VPT; ++v)
+        if (piece(v) < a.cols) near |= near_border(t[v], inv, border) << (8 * v);
+    }
+    if constexpr (MODE == kSilu) {
+      if (st.m >= least) {
+        uint32_t can = 0;
+#pragma unroll
+        for (int v = 0; v < VPT; ++v)
+          if (piece(v) < a.cols)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) can |= fabsf(at(t[v], i)) >= least ? 1u << (8 * v + i) : 0u;
+        for (; can; can &= can - 1) fin.candidate(ri, __ffs(int(can)) - 1);
+      }
+      fin.end(ri, near, false);
+      __syncthreads();
+      fin.settle();
+    } else {
+      if (near) fin.set_codes(ri, near, fin.m64);
+      fin.norm_scale(ri, f);
+    }
+  } else {
+    double m64 = fin.m64;
+    if constexpr (MODE == kSilu) {
+      for (int v = 0; piece(v) < a.cols; ++v) {
+        Stats<T> unused;
+        load_eval8<T, MODE>(a, row, piece(v), t[0], unused);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (fabsf(at(t[0], i)) >= least) fin.candidate(ri, 8 * v + i);
+      }
+      fin.end(ri, 0, false);
+      __syncthreads();
+      m64 = __longlong_as_double((long long)top64[0]);  // the first row's slot
+      fin.settle();
+    } else {
+      fin.norm_scale(ri, f);
+    }
+    for (int v = 0; piece(v) < a.cols; ++v) {
+      const int c = piece(v);
       if constexpr (MODE == kAddNorm) {  // h is stored: the sum must not be taken again
 #pragma unroll
-        for (int i = 0; i < 8; ++i) tt[i] = c + i < a.cols ? float(row.t64(c + i)) : 0.f;
+        for (int i = 0; i < 4; ++i)
+          t[0][i] = pair(c + 2 * i < a.cols ? float(row.t64(c + 2 * i)) : 0.f,
+                         c + 2 * i + 1 < a.cols ? float(row.t64(c + 2 * i + 1)) : 0.f);
       } else {
-        eval8<T, MODE>(a, row, c, tt, unused);
+        Stats<T> unused;
+        load_eval8<T, MODE>(a, row, c, t[0], unused);
       }
+      float most = 0.f;
+      store_codes(q, c, a.cols, a.vec_q, quantise8(t[0], inv, border, most));
+      if (most > first_test(border))
+        for (uint32_t b = near_border(t[0], inv, border); b; b &= b - 1) {
+          const int at = c + __ffs(int(b)) - 1;
+          if (at < a.cols) q[at] = int8_t(code64<T, MODE>(row, at, m64));
+        }
     }
-    int code[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float z = (VPT ? t[VPT ? v : 0][i] : tt[i]) * inv;
-      const float n = rintf(z);
-      code[i] = int(n);
-      if (slow || fabsf(fabsf(z - n) - 0.5f) < kBand<MODE>)
-        code[i] = c + i < a.cols && m64 > 0.0 ? int(rint(127.0 * row.t64(c + i) / m64)) : 0;
-    }
-    store_codes(q, c, a.cols, a.vec_q, code);
   }
+}
+
+cudaLaunchConfig_t launch_config(unsigned grid, unsigned block, size_t smem, cudaStream_t s, cudaLaunchAttribute* pdl) {
+  pdl->id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  pdl->val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = pdl;
+  cfg.numAttrs = 1;
+  return cfg;
 }
 
 template <class T, int MODE, int THREADS, int VPT>
-cudaError_t launch(const RowArgs& a, int rows, cudaStream_t s) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(rows));
-  cfg.blockDim = dim3(THREADS);
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
+cudaError_t launch_row(const RowArgs& a, cudaStream_t s) {
+  cudaLaunchAttribute pdl;
+  const cudaLaunchConfig_t cfg = launch_config(unsigned(a.rows), THREADS, 0, s, &pdl);
   return cudaLaunchKernelEx(&cfg, &i8_row_kernel<T, MODE, THREADS, VPT>, a);
 }
 
+template <class T, int MODE, int MOST, int BLOCKS>
+cudaError_t launch_rows(const RowArgs& a, int threads, int sms, cudaStream_t s) {
+  auto* kern = &i8_rows_kernel<T, MODE, MOST, BLOCKS>;
+  constexpr int kBytes = kPieces * 16 * (MODE == kNorm ? 1 : 2);  // a thread's share
+  static gpu::SmemOptIn optin;
+  if (const cudaError_t e = optin.ensure(reinterpret_cast<const void*>(kern), size_t(kBytes) * MOST); e != cudaSuccess)
+    return e;
+  const int fit = std::min(MOST * BLOCKS / threads, 16);
+  cudaLaunchAttribute pdl;
+  const cudaLaunchConfig_t cfg = launch_config(unsigned(std::min(a.rows, sms * fit)), unsigned(threads),
+                                               size_t(kBytes) * threads, s, &pdl);
+  return cudaLaunchKernelEx(&cfg, kern, a);
+}
 template <class T, int MODE>
-cudaError_t run(const RowArgs& a, int rows, cudaStream_t s) {
+cudaError_t launch_rows(const RowArgs& a, int sms, cudaStream_t s) {
+  const int threads = ceil_div(a.cols, 32 * 8 * kPieces) * 32;
+  if (threads <= 128) return launch_rows<T, MODE, 128, 6>(a, threads, sms, s);
+  if (threads <= 256) return launch_rows<T, MODE, 256, 3>(a, threads, sms, s);
+  if (threads <= 448) return launch_rows<T, MODE, 448, 2>(a, threads, sms, s);
+  return launch_rows<T, MODE, 1024, 1>(a, threads, sms, s);
+}
+
+template <class T, int MODE>
+cudaError_t run(const RowArgs& a, cudaStream_t s) {
+  const gpu::Target* d = gpu::this_device();
+  if (!d) return cudaErrorInvalidDevice;
   const int c = a.cols;
-  if (c <= 1024) return launch<T, MODE, 128, 1>(a, rows, s);
-  if (c <= 2048) return launch<T, MODE, 256, 1>(a, rows, s);
-  if (c <= 4096) return launch<T, MODE, 256, 2>(a, rows, s);
-  if (c <= 8192) return launch<T, MODE, 512, 2>(a, rows, s);
-  if (c <= 16384) return launch<T, MODE, 512, 4>(a, rows, s);
-  if (c <= 32768) return launch<T, MODE, 1024, 4>(a, rows, s);
-  return launch<T, MODE, 1024, 0>(a, rows, s);
+  if (c > 32768) return launch_row<T, MODE, 1024, 0>(a, s);
+  if (a.vec && a.vec_q && c % 8 == 0 && a.rows > 2 * d->sms) return launch_rows<T, MODE>(a, d->sms, s);
+  if (c <= 1024) return launch_row<T, MODE, 128, 1>(a, s);
+  if (c <= 4096) return launch_row<T, MODE, 512, 1>(a, s);
+  if (c <= 8192) return launch_row<T, MODE, 1024, 1>(a, s);
+  if (c <= 16384) return launch_row<T, MODE, 1024, 2>(a, s);
+  return launch_row<T, MODE, 1024, 4>(a, s);
 }
 
 bool aligned16(const void* p, long long ld) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 8 == 0; }
 
 RowArgs make_args(const RowOp& o) {
   RowArgs a{};
+  a.rows = o.rows;
   a.cols = o.cols;
   a.x = o.x;
   a.ldx = o.ldx;
@@ -349,14 +751,14 @@ cudaError_t rmsnorm(const RowOp& o, cudaStream_t s) {
   if (o.rows == 0) return cudaSuccess;
   const RowArgs a = make_args(o);
   if (o.residual)
-    return o.bf16 ? run<__nv_bfloat16, kAddNorm>(a, o.rows, s) : run<__half, kAddNorm>(a, o.rows, s);
-  return o.bf16 ? run<__nv_bfloat16, kNorm>(a, o.rows, s) : run<__half, kNorm>(a, o.rows, s);
+    return o.bf16 ? run<__nv_bfloat16, kAddNorm>(a, s) : run<__half, kAddNorm>(a, s);
+  return o.bf16 ? run<__nv_bfloat16, kNorm>(a, s) : run<__half, kNorm>(a, s);
 }
 
 cudaError_t silu_mul(const RowOp& o, cudaStream_t s) {
   if (o.rows == 0) return cudaSuccess;
   const RowArgs a = make_args(o);
-  return o.bf16 ? run<__nv_bfloat16, kSilu>(a, o.rows, s) : run<__half, kSilu>(a, o.rows, s);
+  return o.bf16 ? run<__nv_bfloat16, kSilu>(a, s) : run<__half, kSilu>(a, s);
 }
 
 }  // namespace aegis::i8

@@ -147,6 +147,30 @@ def test_product_leaves_what_is_between_the_rows(ops, M, N, ldc, out):
     assert (c == 7.0).all()
 
 
+def test_strides_of_every_kind(ops):
+    """Rows of a larger tensor are read in place; other patterns are copied; vectors may be strided."""
+    import torch
+    a, w, sa, sw, b = make(torch, 21, 33, 130, 200, 0, 0, torch.bfloat16)
+    want = ops.matmul_i8(a, w, sa, sw, b)
+    wide = torch.zeros(33, 512, device="cuda", dtype=torch.int8)
+    wide[:, 16:216], wide[:, 300:500] = a, a
+    every2 = torch.zeros(260, 400, device="cuda", dtype=torch.int8)
+    every2[::2, ::2] = w
+    strided = torch.zeros(130, 3, device="cuda")
+    strided[:, 1] = sw
+    for x in (wide[:, 16:216], wide[:, 300:500], a.t().contiguous().t()):
+        for y in (w, w.t().contiguous().t(), every2[::2, ::2]):
+            assert torch.equal(ops.matmul_i8(x, y, sa, strided[:, 1], b), want)
+    row = a[:1].expand(33, 200)
+    assert torch.equal(ops.matmul_i8(row, w, sa[:1].expand(33), sw, b),
+                       ops.matmul_i8(a[:1], w, sa[:1], sw, b).expand(33, 130))
+    x = torch.randn(40, 64, device="cuda").half()
+    g = torch.randn(64, 2, device="cuda").half()
+    q, s, h = ops.add_rmsnorm_i8(x.t(), x.t().contiguous(), g[:40, 0], 1e-5)
+    q2, s2, h2 = ops.add_rmsnorm_i8(x.t().contiguous(), x.t().contiguous(), g[:40, 0].contiguous(), 1e-5)
+    assert torch.equal(q, q2) and torch.equal(s, s2) and torch.equal(h, h2)
+
+
 def test_product_scales_that_are_not_finite(ops):
     import torch
     a, w, sa, sw, _ = make(torch, 9, 20, 40, 128)
@@ -173,7 +197,9 @@ def check_norm(torch, q, s, h, w, eps):
 
 
 ROWS = [(1, 1), (1, 8), (3, 7), (5, 64), (2, 1000), (4, 1024), (3, 1025), (2, 2048), (5, 4096), (3, 4097), (2, 8192),
-        (2, 14336), (2, 16385), (1, 28672), (3, 32768), (2, 32769), (2, 40001), (700, 896)]
+        (2, 14336), (2, 16385), (1, 28672), (3, 32768), (2, 32769), (2, 40001), (700, 896),
+        # more rows than blocks
+        (9000, 100), (4800, 1031), (2500, 4096), (700, 4105), (700, 9000), (400, 17000)]
 
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
@@ -236,22 +262,38 @@ def test_codes_at_the_borders(ops, cols):
 @pytest.mark.parametrize("cols", [64, 4097, 40000])
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
 def test_rows_that_are_zero_or_not_finite(ops, dtype, cols):
+    zero_or_not_finite(ops, dtype, cols, 8)
+
+
+@pytest.mark.parametrize("rows,cols", [(6000, 64), (5000, 1024), (3000, 4096), (800, 12000)])
+def test_zero_and_not_finite_rows_among_many(ops, rows, cols):
+    zero_or_not_finite(ops, "bfloat16", cols, rows)
+
+
+def zero_or_not_finite(ops, dtype, cols, rows):
     import torch
     dt = getattr(torch, dtype)
     g = gen(torch, cols)
-    x = torch.randn(8, cols, device="cuda", generator=g).to(dt)
+    x = torch.randn(rows, cols, device="cuda", generator=g).to(dt)
     w = torch.ones(cols, device="cuda").to(dt)
     w[0] = 0
-    x[1] = 0
-    x[2, cols // 2] = float("nan")
-    x[3, cols - 1] = float("inf")
-    x[4, 0] = -float("inf")  # times a weight of 0
+    x[1::8] = 0
+    x[2::8, cols // 2] = float("nan")
+    x[3::8, cols - 1] = float("inf")
+    x[4::8, 0] = -float("inf")  # times a weight of 0
+    kind = torch.arange(rows, device="cuda") % 8
     for q, s in (ops.rmsnorm_i8(x, w, 1e-5), ops.silu_mul_i8(x, torch.ones_like(x)),
                  ops.silu_mul_i8(torch.ones_like(x), x), ops.add_rmsnorm_i8(x, torch.zeros_like(x), w, 1e-5)[:2]):
-        assert (q[1] == 0).all() and s[1] == 0
-        assert (q[2:5] == 0).all() and s[2:5].isnan().all()
-        rest = torch.tensor([0, 5, 6, 7], device="cuda")
+        assert (q[kind == 1] == 0).all() and (s[kind == 1] == 0).all()
+        bad = (kind >= 2) & (kind <= 4)
+        assert (q[bad] == 0).all() and s[bad].isnan().all()
+        rest = (kind == 0) | (kind >= 5)
         assert s[rest].isfinite().all() and (q[rest].abs().amax(dim=1) == 127).all()
+    q, s = ops.silu_mul_i8(x, torch.ones_like(x))
+    xd = x[rest].double()
+    check_codes(torch, q[rest], xd / (1 + torch.exp(-xd)))
+    q, s = ops.rmsnorm_i8(x, w, 1e-5)
+    check_norm(torch, q[rest], s[rest], x[rest], w, 1e-5)
     big = torch.full((1, cols), 6e4, device="cuda").half()  # the sum leaves f16's range
     q, s, h = ops.add_rmsnorm_i8(big, big, torch.ones(cols, device="cuda").half(), 1e-5)
     assert h.isinf().all() and s.isnan().all() and (q == 0).all()
