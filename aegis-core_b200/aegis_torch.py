@@ -34,6 +34,7 @@ while gradients are recorded.
 """
 from __future__ import annotations
 
+import os
 import threading
 
 import torch
@@ -102,8 +103,7 @@ def _(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
 
 
 # ---------------------------------------------------------------- 8-bit operators
-_DTYPE_CODE = {torch.float16: i8.DTYPE_F16, torch.bfloat16: i8.DTYPE_BF16, torch.float32: i8.DTYPE_F32}
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_OUT_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 
 _defs = torch.library.Library("aegis", "FRAGMENT")
 _defs.define("matmul_i8(Tensor a, Tensor w, Tensor a_scale, Tensor w_scale, Tensor? bias=None, *, "
@@ -113,21 +113,6 @@ _defs.define("add_rmsnorm_i8(Tensor x, Tensor residual, Tensor weight, float eps
 _defs.define("silu_mul_i8(Tensor gate, Tensor up) -> (Tensor, Tensor)")
 _defs.define("mlp_i8(Tensor x, Tensor residual, Tensor norm_weight, float eps, Tensor w_gate_up, Tensor s_gate_up, "
              "Tensor w_down, Tensor s_down) -> (Tensor, Tensor)")
-
-
-def _rows(t: torch.Tensor):
-    """(tensor, row stride) of a 2-D operand whose rows are contiguous and do not overlap, else of a copy."""
-    st0, st1 = t.stride()
-    rows, cols = t.shape
-    if (st1 == 1 or cols <= 1) and (st0 >= cols or rows <= 1):
-        # A single row has no stride of its own: one that every kernel can take.
-        return t, (st0 if rows > 1 else (cols + 15) // 16 * 16)
-    t = t.contiguous()
-    return t, max(cols, 1)
-
-
-def _vector(t: torch.Tensor) -> torch.Tensor:
-    return t if t.is_contiguous() else t.contiguous()
 
 
 def _no_grad(name: str, *tensors) -> None:
@@ -166,7 +151,7 @@ def _check_matmul_i8(a, w, a_scale, w_scale, bias, out_dtype):
     _f32_vector(name, "w_scale", w_scale, w.shape[0])
     if out_dtype is None:
         out_dtype = bias.dtype if bias is not None else torch.bfloat16
-    if out_dtype not in _DTYPE_CODE:
+    if out_dtype not in _OUT_DTYPES:
         raise TypeError(f"aegis::matmul_i8: out_dtype must be float16, bfloat16 or float32, not {out_dtype}")
     if bias is not None:
         if bias.dtype != out_dtype:
@@ -176,26 +161,6 @@ def _check_matmul_i8(a, w, a_scale, w_scale, bias, out_dtype):
     _same_device(name, a, w, a_scale, w_scale, bias)
     _no_grad(name, a_scale, w_scale, bias)
     return out_dtype
-
-
-def _matmul_i8(a, w, a_scale, w_scale, bias=None, *, out_dtype=None):
-    out_dtype = _check_matmul_i8(a, w, a_scale, w_scale, bias, out_dtype)
-    M, K = a.shape
-    N = w.shape[0]
-    dev = a.get_device()
-    out = torch.empty((M, N), dtype=out_dtype, device=a.device)
-    if M and N:
-        a, lda = _rows(a)
-        w, ldw = _rows(w)
-        a_scale, w_scale = _vector(a_scale), _vector(w_scale)
-        if bias is not None:
-            bias = _vector(bias)
-        st = i8.load().aegis_i8_gemm(dev, _raw_stream(dev), _DTYPE_CODE[out_dtype], M, N, K, a.data_ptr(), lda,
-                                     w.data_ptr(), ldw, a_scale.data_ptr(), w_scale.data_ptr(),
-                                     None if bias is None else bias.data_ptr(), out.data_ptr(), N)
-        if st:
-            i8.check(st, "aegis::matmul_i8")
-    return out
 
 
 def _matmul_i8_meta(a, w, a_scale, w_scale, bias=None, *, out_dtype=None):
@@ -236,36 +201,9 @@ def _check_norm(name, x, residual, weight, eps):
     _no_grad(name, x, residual, weight)
 
 
-def _norm(name, x, residual, weight, eps):
-    _check_norm(name, x, residual, weight, eps)
-    q, scale = _empty_codes(x)
-    h = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    rows, cols = x.shape
-    if rows:
-        dev = x.get_device()
-        x, ldx = _rows(x)
-        r, ldr = (None, 0) if residual is None else _rows(residual)
-        weight = _vector(weight)
-        st = i8.load().aegis_i8_rmsnorm(dev, _raw_stream(dev), _DTYPE_CODE[x.dtype], rows, cols, x.data_ptr(), ldx,
-                                        None if r is None else r.data_ptr(), ldr, weight.data_ptr(), eps,
-                                        None if h is None else h.data_ptr(), cols, q.data_ptr(), q.stride(0),
-                                        scale.data_ptr())
-        if st:
-            i8.check(st, f"aegis::{name}")
-    return q, scale, h
-
-
-def _rmsnorm_i8(x, weight, eps):
-    return _norm("rmsnorm_i8", x, None, weight, eps)[:2]
-
-
 def _rmsnorm_i8_meta(x, weight, eps):
     _check_norm("rmsnorm_i8", x, None, weight, eps)
     return _empty_codes(x)
-
-
-def _add_rmsnorm_i8(x, residual, weight, eps):
-    return _norm("add_rmsnorm_i8", x, residual, weight, eps)
 
 
 def _add_rmsnorm_i8_meta(x, residual, weight, eps):
@@ -277,21 +215,6 @@ def _check_silu_mul(gate, up):
     _check_rows("silu_mul_i8", gate, up, "up")
     _same_device("silu_mul_i8", gate, up)
     _no_grad("silu_mul_i8", gate, up)
-
-
-def _silu_mul_i8(gate, up):
-    _check_silu_mul(gate, up)
-    q, scale = _empty_codes(gate)
-    rows, cols = gate.shape
-    if rows:
-        dev = gate.get_device()
-        gate, ldg = _rows(gate)
-        up, ldu = _rows(up)
-        st = i8.load().aegis_i8_silu_mul(dev, _raw_stream(dev), _DTYPE_CODE[gate.dtype], rows, cols, gate.data_ptr(),
-                                         ldg, up.data_ptr(), ldu, q.data_ptr(), q.stride(0), scale.data_ptr())
-        if st:
-            i8.check(st, "aegis::silu_mul_i8")
-    return q, scale
 
 
 def _silu_mul_i8_meta(gate, up):
@@ -319,39 +242,18 @@ def _check_mlp(x, residual, norm_weight, eps, w_gate_up, s_gate_up, w_down, s_do
     _no_grad(name, s_gate_up, s_down)
 
 
-def _mlp_i8(x, residual, norm_weight, eps, w_gate_up, s_gate_up, w_down, s_down):
-    _check_mlp(x, residual, norm_weight, eps, w_gate_up, s_gate_up, w_down, s_down)
-    M, K = x.shape
-    F = w_down.shape[1]
-    y = torch.empty((M, K), dtype=x.dtype, device=x.device)
-    h = torch.empty((M, K), dtype=x.dtype, device=x.device)
-    if M:
-        dev = x.get_device()
-        x, ldx = _rows(x)
-        r, ldr = _rows(residual)
-        w1, ld1 = _rows(w_gate_up)
-        w2, ld2 = _rows(w_down)
-        g, s1, s2 = _vector(norm_weight), _vector(s_gate_up), _vector(s_down)
-        nbytes = i8.mlp_workspace(M, K, F)
-        ws = torch.empty((nbytes,), dtype=torch.uint8, device=x.device)  # torch's allocator: 512-byte aligned
-        st = i8.load().aegis_i8_mlp(dev, _raw_stream(dev), _DTYPE_CODE[x.dtype], M, K, F, x.data_ptr(), ldx,
-                                    r.data_ptr(), ldr, g.data_ptr(), eps, w1.data_ptr(), ld1, s1.data_ptr(),
-                                    w2.data_ptr(), ld2, s2.data_ptr(), h.data_ptr(), K, y.data_ptr(), K,
-                                    ws.data_ptr(), nbytes)
-        if st:
-            i8.check(st, "aegis::mlp_i8")
-    return y, h
-
-
 def _mlp_i8_meta(x, residual, norm_weight, eps, w_gate_up, s_gate_up, w_down, s_down):
     _check_mlp(x, residual, norm_weight, eps, w_gate_up, s_gate_up, w_down, s_down)
     return x.new_empty(x.shape), x.new_empty(x.shape)
 
 
-for _name, _cuda, _meta in (("matmul_i8", _matmul_i8, _matmul_i8_meta),
-                            ("rmsnorm_i8", _rmsnorm_i8, _rmsnorm_i8_meta),
-                            ("add_rmsnorm_i8", _add_rmsnorm_i8, _add_rmsnorm_i8_meta),
-                            ("silu_mul_i8", _silu_mul_i8, _silu_mul_i8_meta),
-                            ("mlp_i8", _mlp_i8, _mlp_i8_meta)):
-    _defs.impl(_name, _cuda, "CUDA")
+for _name, _meta in (("matmul_i8", _matmul_i8_meta), ("rmsnorm_i8", _rmsnorm_i8_meta),
+                     ("add_rmsnorm_i8", _add_rmsnorm_i8_meta), ("silu_mul_i8", _silu_mul_i8_meta),
+                     ("mlp_i8", _mlp_i8_meta)):
     _defs.impl(_name, _meta, "Meta")
+
+# The CUDA implementations (csrc/i8/torch_ops.cpp) call libaegis_i8.so.
+_TORCH_LIB = os.path.join(ac.HERE, "build", "libaegis_torch_i8.so")
+if not os.path.exists(_TORCH_LIB):
+    raise FileNotFoundError(f"{_TORCH_LIB} is not built: run `make -C aegis-core_b200` (or __graft_entry__.build())")
+torch.ops.load_library(_TORCH_LIB)

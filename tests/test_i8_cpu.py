@@ -208,15 +208,3 @@ def test_gradients_may_be_off():
     x = meta(4, 8).requires_grad_()
     with torch.no_grad():
         assert ops.rmsnorm_i8(x, meta(8), 1e-5)[0].shape == (4, 8)
-
-
-def test_rows_and_their_strides():
-    t = torch.zeros(6, 40, dtype=torch.int8)
-    assert aegis_torch._rows(t) == (t, 40)
-    v = t[:, :33]
-    assert aegis_torch._rows(v)[1] == 40 and aegis_torch._rows(v)[0] is v
-    one = t[:1, :33]
-    assert aegis_torch._rows(one)[1] == 48  # a single row: any stride, so one of 16 bytes
-    for odd in (t.t(), t[:, ::2], t[:1].expand(4, 40)):
-        got, ld = aegis_torch._rows(odd)
-        assert got.is_contiguous() and ld == odd.shape[1]
