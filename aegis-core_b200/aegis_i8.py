@@ -8,7 +8,6 @@ library is missing, ``load()`` raises.
 from __future__ import annotations
 
 import ctypes
-import functools
 import json
 import os
 from ctypes import POINTER, c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p
@@ -26,16 +25,19 @@ _SIGNATURES = {
     "aegis_i8_last_error_string": (c_char_p, []),
     "aegis_i8_synchronize": (c_int, [c_int, c_void_p]),
     "aegis_i8_gemm": (c_int, [c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_int64, c_void_p, c_int64,
-                              c_void_p, c_void_p, c_void_p, c_void_p, c_int64]),
+                              c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_size_t]),
+    "aegis_i8_gemm_workspace": (c_int, [c_int, c_int, c_int, c_void_p, c_int64, c_void_p, c_int64,
+                                        POINTER(c_size_t)]),
     "aegis_i8_rmsnorm": (c_int, [c_int, c_void_p, c_int, c_int, c_int, c_void_p, c_int64, c_void_p, c_int64,
                                  c_void_p, c_float, c_void_p, c_int64, c_void_p, c_int64, c_void_p]),
     "aegis_i8_silu_mul": (c_int, [c_int, c_void_p, c_int, c_int, c_int, c_void_p, c_int64, c_void_p, c_int64,
                                   c_void_p, c_int64, c_void_p]),
-    "aegis_i8_mlp_workspace": (c_int, [c_int, c_int, c_int, POINTER(c_size_t)]),
+    "aegis_i8_mlp_workspace": (c_int, [c_int, c_int, c_int, c_void_p, c_int64, c_void_p, c_int64,
+                                       POINTER(c_size_t)]),
     "aegis_i8_mlp": (c_int, [c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_int64, c_void_p, c_int64,
                              c_void_p, c_float, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p,
                              c_int64, c_void_p, c_int64, c_void_p, c_size_t]),
-    "aegis_i8_gemm_plan_json": (c_int, [c_int, c_int, c_int, c_int, c_int, c_char_p, c_size_t, POINTER(c_size_t)]),
+    "aegis_i8_gemm_plan_json": (c_int, [c_int, c_int, c_int, c_int, c_char_p, c_size_t, POINTER(c_size_t)]),
 }
 
 _lib = None
@@ -71,18 +73,25 @@ def synchronize(device: int, stream: int) -> None:
     check(load().aegis_i8_synchronize(device, stream), "aegis_i8_synchronize")
 
 
-@functools.lru_cache(maxsize=4096)
-def mlp_workspace(M: int, K: int, F: int) -> int:
-    """Bytes of workspace aegis_i8_mlp needs for these sizes."""
+def gemm_workspace(M: int, N: int, K: int, A: int, lda: int, W: int, ldw: int) -> int:
+    """Bytes of workspace aegis_i8_gemm needs for these operands."""
     n = c_size_t(0)
-    check(load().aegis_i8_mlp_workspace(M, K, F, ctypes.byref(n)), "aegis_i8_mlp_workspace")
+    check(load().aegis_i8_gemm_workspace(M, N, K, A, lda, W, ldw, ctypes.byref(n)), "aegis_i8_gemm_workspace")
     return n.value
 
 
-def gemm_plan(M: int, N: int, K: int, tma: bool = True, sm_count: int = 148) -> dict:
+def mlp_workspace(M: int, K: int, F: int, w_gate_up: int, ld_gate_up: int, w_down: int, ld_down: int) -> int:
+    """Bytes of workspace aegis_i8_mlp needs for these operands."""
+    n = c_size_t(0)
+    check(load().aegis_i8_mlp_workspace(M, K, F, w_gate_up, ld_gate_up, w_down, ld_down, ctypes.byref(n)),
+          "aegis_i8_mlp_workspace")
+    return n.value
+
+
+def gemm_plan(M: int, N: int, K: int, sm_count: int = 148) -> dict:
     """The launch aegis_i8_gemm makes on a device with `sm_count` SMs (needs no GPU)."""
     buf = ctypes.create_string_buffer(512)
     needed = c_size_t(0)
-    check(load().aegis_i8_gemm_plan_json(sm_count, M, N, K, int(tma), buf, len(buf), ctypes.byref(needed)),
+    check(load().aegis_i8_gemm_plan_json(sm_count, M, N, K, buf, len(buf), ctypes.byref(needed)),
           "aegis_i8_gemm_plan_json")
     return json.loads(buf.value.decode())

@@ -126,12 +126,17 @@ size_t up(size_t n, size_t to) { return (n + to - 1) / to * to; }
 
 // The workspace of a feed-forward block.
 struct MlpSpace {
-  size_t q1, s1, gu, q2, s2, bytes;
+  size_t q1, s1, gu, q2, s2, w1, w2, bytes;
   long long ld1, ldgu, ld2;
-  MlpSpace(int M, int K, int F) {
+  bool copy1, copy2;  // the weights' rows need a copy that TMA can address
+  MlpSpace(int M, int K, int F, const void* w_gate_up, int64_t ld_gate_up, const void* w_down, int64_t ld_down) {
     ld1 = (long long)up(size_t(K), 16);
     ldgu = (long long)up(2 * size_t(F), 8);
     ld2 = (long long)up(size_t(F), 16);
+    if (M == 0) {
+      bytes = 0;
+      return;
+    }
     size_t at = 0;
     auto take = [&](size_t n) {
       const size_t was = at;
@@ -143,6 +148,10 @@ struct MlpSpace {
     gu = take(size_t(M) * size_t(ldgu) * 2);
     q2 = take(size_t(M) * size_t(ld2));
     s2 = take(size_t(M) * 4);
+    copy1 = !aegis::i8::tma_rows(w_gate_up, ld_gate_up);
+    copy2 = !aegis::i8::tma_rows(w_down, ld_down);
+    w1 = take(copy1 ? 2 * size_t(F) * aegis::i8::aligned_cols(K) : 0);
+    w2 = take(copy2 ? size_t(K) * aegis::i8::aligned_cols(F) : 0);
     bytes = at;
   }
 };
@@ -176,9 +185,20 @@ int aegis_i8_synchronize(int device, void* stream) {
   return fail(AEGIS_ERR_CUDA, fn, b);
 }
 
+int aegis_i8_gemm_workspace(int M, int N, int K, const void* A, int64_t lda, const void* W, int64_t ldw,
+                            size_t* bytes) {
+  const char* fn = "aegis_i8_gemm_workspace";
+  if (!bytes) return bad(fn, "bytes is NULL");
+  if (!size_ok(M) || !size_ok(N) || K < 0) return bad(fn, "negative size or a size above 2^31 - 2^20");
+  if (K > AEGIS_I8_MAX_K) return bad(fn, "K above AEGIS_I8_MAX_K: the int32 sum could overflow");
+  const aegis::i8::GemmSpace need = aegis::i8::gemm_space(A, lda, W, ldw, M, N, K);
+  *bytes = M == 0 || N == 0 ? 0 : need.w + need.a;
+  return AEGIS_OK;
+}
+
 int aegis_i8_gemm(int device, void* stream, int out_dtype, int M, int N, int K, const void* A, int64_t lda,
                   const void* W, int64_t ldw, const float* a_scale, const float* w_scale, const void* bias, void* C,
-                  int64_t ldc) {
+                  int64_t ldc, void* workspace, size_t workspace_bytes) {
   const char* fn = "aegis_i8_gemm";
   Gemm g;
   g.A = A;
@@ -196,6 +216,13 @@ int aegis_i8_gemm(int device, void* stream, int out_dtype, int M, int N, int K, 
   if (const char* w = check(g, out_dtype)) return bad(fn, w);
   g.out = static_cast<Out>(out_dtype);
   if (M == 0 || N == 0) return AEGIS_OK;
+  const aegis::i8::GemmSpace need = aegis::i8::gemm_space(A, lda, W, ldw, M, N, K);
+  if (need.w + need.a > 0) {
+    if (!workspace || workspace_bytes < need.w + need.a)
+      return fail(AEGIS_ERR_BUFFER_TOO_SMALL, fn, "the workspace is smaller than aegis_i8_gemm_workspace asks for");
+    if (!aligned(workspace, 256)) return bad(fn, "the workspace is not 256-byte aligned");
+  }
+  g.workspace = workspace;
   return on_device(device, fn, [&] { return aegis::i8::gemm(g, static_cast<cudaStream_t>(stream)); });
 }
 
@@ -244,11 +271,12 @@ int aegis_i8_silu_mul(int device, void* stream, int dtype, int rows, int cols, c
   return on_device(device, fn, [&] { return aegis::i8::silu_mul(o, static_cast<cudaStream_t>(stream)); });
 }
 
-int aegis_i8_mlp_workspace(int M, int K, int F, size_t* bytes) {
+int aegis_i8_mlp_workspace(int M, int K, int F, const void* w_gate_up, int64_t ld_gate_up, const void* w_down,
+                           int64_t ld_down, size_t* bytes) {
   const char* fn = "aegis_i8_mlp_workspace";
   if (!bytes) return bad(fn, "bytes is NULL");
   if (const char* w = check_mlp_sizes(M, K, F)) return bad(fn, w);
-  *bytes = MlpSpace(M, K, F).bytes;
+  *bytes = MlpSpace(M, K, F, w_gate_up, ld_gate_up, w_down, ld_down).bytes;
   return AEGIS_OK;
 }
 
@@ -260,7 +288,7 @@ int aegis_i8_mlp(int device, void* stream, int dtype, int M, int K, int F, const
   if (const char* w = check_mlp_sizes(M, K, F)) return bad(fn, w);
   if (!dtype16(dtype)) return bad(fn, "dtype must be AEGIS_DTYPE_F16 or AEGIS_DTYPE_BF16");
   if (M == 0) return AEGIS_OK;
-  const MlpSpace at(M, K, F);
+  const MlpSpace at(M, K, F, w_gate_up, ld_gate_up, w_down, ld_down);
   if (!workspace || workspace_bytes < at.bytes)
     return fail(AEGIS_ERR_BUFFER_TOO_SMALL, fn, "the workspace is smaller than aegis_i8_mlp_workspace asks for");
   if (!aligned(workspace, 256)) return bad(fn, "the workspace is not 256-byte aligned");
@@ -328,9 +356,21 @@ int aegis_i8_mlp(int device, void* stream, int dtype, int M, int K, int F, const
   g2.weights_settled = true;
   if (const char* w = check(g2, dtype)) return bad(fn, w);
 
+  // Copies first: the products may then read them before the row operations end.
   return on_device(device, fn, [&] {
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    cudaError_t e = aegis::i8::rmsnorm(norm, s);
+    cudaError_t e = cudaSuccess;
+    if (at.copy1) {
+      e = aegis::i8::align(w_gate_up, ld_gate_up, 2 * F, K, ws + at.w1, s);
+      g1.W = ws + at.w1;
+      g1.ldw = (long long)aegis::i8::aligned_cols(K);
+    }
+    if (at.copy2 && e == cudaSuccess) {
+      e = aegis::i8::align(w_down, ld_down, K, F, ws + at.w2, s);
+      g2.W = ws + at.w2;
+      g2.ldw = (long long)aegis::i8::aligned_cols(F);
+    }
+    if (e == cudaSuccess) e = aegis::i8::rmsnorm(norm, s);
     if (e == cudaSuccess) e = aegis::i8::gemm(g1, s);
     if (e == cudaSuccess) e = aegis::i8::silu_mul(act, s);
     if (e == cudaSuccess) e = aegis::i8::gemm(g2, s);
@@ -338,16 +378,19 @@ int aegis_i8_mlp(int device, void* stream, int dtype, int M, int K, int F, const
   });
 }
 
-int aegis_i8_gemm_plan_json(int sm_count, int M, int N, int K, int tma, char* buf, size_t buf_len, size_t* needed) {
+int aegis_i8_gemm_plan_json(int sm_count, int M, int N, int K, char* buf, size_t buf_len, size_t* needed) {
   const char* fn = "aegis_i8_gemm_plan_json";
   if (M < 1 || N < 1 || K < 0 || !size_ok(M) || !size_ok(N) || K > AEGIS_I8_MAX_K)
     return bad(fn, "M and N must be from 1 to 2^31 - 2^20, K from 0 to AEGIS_I8_MAX_K");
   if (sm_count < 1 || sm_count > 4096) return bad(fn, "sm_count must be from 1 to 4096");
-  const aegis::i8::GemmPlan p = aegis::i8::plan_gemm(M, N, K, tma != 0 && K > 0, sm_count);
+  const aegis::i8::GemmPlan p = aegis::i8::plan_gemm(M, N, K, sm_count);
+  const char* kernel = p.kernel == aegis::i8::GemmKernel::Pair  ? "pair"
+                       : p.kernel == aegis::i8::GemmKernel::Dot ? "dot"
+                                                                 : "stream";
   char b[256];
   const int n = std::snprintf(b, sizeof b,
                               "{\"kernel\":\"%s\",\"tile_m\":%d,\"tile_n\":%d,\"splits\":%d,\"tiles\":%lld,\"grid\":%lld}",
-                              p.pair ? "pair" : "stream", p.tile_m, p.tile_n, p.splits, p.tiles, p.grid);
+                              kernel, p.tile_m, p.tile_n, p.splits, p.tiles, p.grid);
   if (needed) *needed = size_t(n) + 1;
   if (!buf && buf_len == 0) return AEGIS_OK;
   if (!buf) return bad(fn, "buf is NULL but buf_len is not 0");

@@ -4,6 +4,8 @@
 #include "../gpu_target.h"
 #include "../status.h"
 #include "../tma_map.h"
+#include "i8_align.cuh"
+#include "i8_dot.cuh"
 #include "i8_pair.cuh"
 #include "i8_stream.cuh"
 
@@ -13,42 +15,112 @@ bool tma_rows(const void* p, long long ld) { return (reinterpret_cast<uintptr_t>
 
 namespace {
 
-// Ring depths: about 100 KB for up to 128 tokens, so two CTAs share an SM and
-// one's epilogue overlaps the other's stream; 192 KB for 256 tokens.
-constexpr int stages_for(int nt) { return nt == 16 ? 6 : nt == 32 ? 5 : nt == 64 ? 4 : nt == 128 ? 3 : 4; }
-constexpr int ctas_per_sm(int nt) { return nt <= 128 ? 2 : 1; }
+// The stream kernel's variants, by tokens a tile. Rings of about 100 KB for up to
+// 128 tokens, so two CTAs share an SM and one's epilogue overlaps the other's
+// stream; 192 KB for 256. Measured on a B200 (K = 4096, one wave of CTAs): the time
+// of a stage, which is the copies' latency over the ring's depth as long as DRAM
+// keeps up, and what joining the slices of a cluster costs.
+struct StreamVariant {
+  int tokens, group, stages, ctas_per_sm;  // group: k-blocks a stage
+  double stage_us, join_us;
+};
+constexpr StreamVariant kStream[] = {
+    {16, 2, 3, 2, 0.39, 1.0}, {32, 2, 2, 2, 0.6, 1.3},  {64, 2, 2, 2, 0.77, 1.8},
+    {128, 1, 3, 2, 0.58, 2.5}, {256, 1, 4, 1, 0.86, 4.0},
+};
+constexpr const StreamVariant& variant(int tokens) {
+  for (const StreamVariant& v : kStream)
+    if (v.tokens == tokens) return v;
+  return kStream[0];
+}
+constexpr int group_for(int nt) { return variant(nt).group; }
+constexpr int stages_for(int nt) { return variant(nt).stages; }
 
 }  // namespace
 
-GemmPlan plan_gemm(int M, int N, int K, bool tma, int sms) {
+// The estimates below (microseconds) only have to order the choices; they are
+// within 15% of what was measured over M = 16 .. 2048, N = 896 .. 28672, K = 896 ..
+// 14336. Times without what every launch costs (about 5).
+GemmPlan plan_gemm(int M, int N, int K, int sms) {
   GemmPlan p;
   const int kb = ceil_div(K, BK);
+  if (K > 0 && M <= kDotTokens) {
+    // Where the loads of a warp's share of K are all on their way at once and no
+    // second wave of warps (16 an SM) follows. B200, us, this kernel and the
+    // stream kernel: 1 x 4096 x 4096 6.1, 7.5; 4 x 4096 x 4096 6.7, 7.6; 8 x 4096 x
+    // 4096 8.4, 7.7; 1 x 896 x 4864 4.1, 5.9; 1 x 4096 x 14336 14.1, 13.0;
+    // 1 x 14336 x 4096 17.0, 13.8.
+    const long long groups = ceil_div(N, kDotChannels), warps = 16ll * sms;
+    int parts = 1;
+    while (parts < kDotWarps && groups * parts * 2 <= warps && K >= 1024 * parts) parts *= 2;
+    if (groups * parts <= warps && K <= parts * (M <= 4 ? 2048 : 1024)) {
+      p.kernel = GemmKernel::Dot;
+      p.tile_m = M;
+      p.tile_n = kDotChannels;
+      p.tiles = groups;
+      p.splits = parts;
+      p.grid = ceil_div(groups, (long long)(kDotWarps / parts));
+      return p;
+    }
+  }
+  // CTA pairs: 256 x 256 tiles, 0.36 us a k-block, and 5 more for a wave's first
+  // copies and last epilogue.
   const long long pair_tiles = (long long)ceil_div(M, 256) * ceil_div(N, 256);
-  if (tma && M > 128 && pair_tiles >= sms / 3) {
-    p.pair = true;
+  const double dram_us = double(N) * K / 6.5e6;
+  double best = 1e300;
+  if (K > 0 && M > 64) {
+    best = std::max(dram_us, 5.0 + 0.36 * kb * double(ceil_div(pair_tiles, (long long)std::max(1, sms / 2))));
+    p.kernel = GemmKernel::Pair;
     p.tile_m = p.tile_n = 256;
     p.tiles = pair_tiles;
     p.grid = 2 * pair_tiles;
-    return p;
   }
-  p.tile_n = BN;
-  p.tile_m = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
-  p.tiles = (long long)ceil_div(M, p.tile_m) * ceil_div(N, BN);
-  const long long slots = (long long)sms * ctas_per_sm(p.tile_m);
-  while (p.splits < 8 && p.tiles * p.splits * 2 <= slots && kb >= 4 * p.splits) p.splits *= 2;
-  p.grid = p.tiles * p.splits;
+  for (const StreamVariant& v : kStream) {
+    if (v.tokens > 16 && v.tokens >= 2 * M) break;  // a smaller tile holds them all
+    const long long token_tiles = ceil_div(M, v.tokens), slots = (long long)sms * v.ctas_per_sm;
+    const int steps = ceil_div(kb, v.group);
+    for (int S = 1; S <= 8 && S <= std::max(1, steps); S *= 2) {
+      // Clusters of 4 and 8 leave some of a GPC's SMs unused: about an eighth.
+      const long long room = S >= 4 ? slots * 7 / 8 : slots;
+      int rows = BN;
+      long long tiles = token_tiles * ceil_div(N, rows);
+      if (S > 1 && tiles * S > room) continue;
+      if (S == 1 && tiles < room && dram_us > steps * v.stage_us) {
+        // DRAM bounds it: narrower tiles while one wave holds them, so every SM gets the same share.
+        const long long each = ceil_div((long long)N, room / token_tiles);
+        rows = int(std::min<long long>(BN, (each + 7) / 8 * 8));
+        tiles = token_tiles * ceil_div(N, rows);
+      }
+      const double waves = double(ceil_div(tiles * S, room));
+      // Memory: DRAM once, or L2 once a token tile. It hides the stages' time, or the
+      // other way round, for the most part. A token's store takes 0.02 us, another wave 3.
+      const double memory_us = std::max(dram_us, dram_us * 0.6 * double(token_tiles));
+      const double stages_us = waves * ceil_div(steps, S) * v.stage_us;
+      const double us = std::max(memory_us, stages_us) + 0.25 * std::min(memory_us, stages_us) +
+                        (S > 1 ? v.join_us * (0.9 + 0.1 * double(token_tiles)) : 0.0) + 0.02 * v.tokens + 3.0 * (waves - 1.0);
+      if (us < best) {
+        best = us;
+        p.kernel = GemmKernel::Stream;
+        p.tile_m = v.tokens;
+        p.tile_n = rows;
+        p.splits = S;
+        p.tiles = tiles;
+        p.grid = tiles * S;
+      }
+    }
+  }
   return p;
 }
 
 namespace {
 
-template <int NT, int LOAD>
+template <int NT>
 cudaError_t launch_stream(const CUtensorMap& tw, const CUtensorMap& ta, const StreamArgs& a, unsigned grid,
                           cudaStream_t s) {
-  constexpr int ST = stages_for(NT);
-  auto* kern = &i8_stream_kernel<NT, ST, LOAD>;
+  constexpr int ST = stages_for(NT), G = group_for(NT);
+  auto* kern = &i8_stream_kernel<NT, ST, G>;
   static gpu::SmemOptIn optin;
-  constexpr size_t smem = size_t(StreamLayout<NT, ST>::ALLOC);
+  constexpr size_t smem = size_t(StreamLayout<NT, ST, G>::ALLOC);
   if (const cudaError_t e = optin.ensure(reinterpret_cast<const void*>(kern), smem); e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid);
@@ -67,15 +139,34 @@ cudaError_t launch_stream(const CUtensorMap& tw, const CUtensorMap& ta, const St
   return cudaLaunchKernelEx(&cfg, kern, tw, ta, a);
 }
 
-template <int LOAD>
+template <int MT>
+cudaError_t launch_dot(const DotArgs& a, unsigned grid, cudaStream_t s) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kDotThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // the kernel waits (griddepcontrol.wait)
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, &i8_dot_kernel<MT>, a);
+}
+cudaError_t launch_dot(const DotArgs& a, unsigned grid, cudaStream_t s) {
+  if (a.M == 1) return launch_dot<1>(a, grid, s);
+  if (a.M == 2) return launch_dot<2>(a, grid, s);
+  if (a.M <= 4) return launch_dot<4>(a, grid, s);
+  return launch_dot<8>(a, grid, s);
+}
+
 cudaError_t launch_stream(int nt, const CUtensorMap& tw, const CUtensorMap& ta, const StreamArgs& a, unsigned grid,
                           cudaStream_t s) {
   switch (nt) {
-    case 16: return launch_stream<16, LOAD>(tw, ta, a, grid, s);
-    case 32: return launch_stream<32, LOAD>(tw, ta, a, grid, s);
-    case 64: return launch_stream<64, LOAD>(tw, ta, a, grid, s);
-    case 128: return launch_stream<128, LOAD>(tw, ta, a, grid, s);
-    default: return launch_stream<256, LOAD>(tw, ta, a, grid, s);
+    case 16: return launch_stream<16>(tw, ta, a, grid, s);
+    case 32: return launch_stream<32>(tw, ta, a, grid, s);
+    case 64: return launch_stream<64>(tw, ta, a, grid, s);
+    case 128: return launch_stream<128>(tw, ta, a, grid, s);
+    default: return launch_stream<256>(tw, ta, a, grid, s);
   }
 }
 
@@ -105,7 +196,49 @@ cudaError_t launch_pair(const CUtensorMap& ta, const CUtensorMap& tw, const Pair
 
 constexpr long long kMaxPairUnits = 1ll << 29;  // umma's raster arithmetic is 32-bit
 
+// Rows that TMA can address as they are, or a copy of them.
+struct Rows {
+  const void* p;
+  long long ld;
+  int K;
+};
+// Copies of W (N rows) and of A (M rows), where asked for, in one launch.
+cudaError_t align_rows(Rows* w, int N, void* w_copy, Rows* t, int M, void* t_copy, cudaStream_t s) {
+  AlignArgs a{};
+  a.K = w_copy ? w->K : t->K;
+  a.padded = int(aligned_cols(a.K));
+  a.segments = ceil_div(a.padded, 128 * kAlignWords);
+  if (w_copy) a.job[0] = {static_cast<const int8_t*>(w->p), w->ld, static_cast<int8_t*>(w_copy), (long long)N * a.segments};
+  if (t_copy) a.job[1] = {static_cast<const int8_t*>(t->p), t->ld, static_cast<int8_t*>(t_copy), (long long)M * a.segments};
+  const long long grid = ceil_div(a.job[0].tasks + a.job[1].tasks, (long long)(kAlignThreads / 32));
+  if (grid > 0x7fffffffll) return cudaErrorInvalidValue;
+  if (w_copy) *w = Rows{w_copy, a.padded, a.padded};
+  if (t_copy) *t = Rows{t_copy, a.padded, a.padded};
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(grid));
+  cfg.blockDim = dim3(kAlignThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // the kernel waits (griddepcontrol.wait)
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, &i8_align_kernel, a);
+}
+
 }  // namespace
+
+cudaError_t align(const void* src, long long ld, int rows, int K, void* dst, cudaStream_t s) {
+  Rows r{src, ld, K};
+  return align_rows(&r, rows, dst, nullptr, 0, nullptr, s);
+}
+
+GemmSpace gemm_space(const void* A, long long lda, const void* W, long long ldw, int M, int N, int K) {
+  GemmSpace sp;
+  sp.w = K > 0 && !tma_rows(W, ldw) ? size_t(N) * aligned_cols(K) : 0;
+  sp.a = K > 0 && !tma_rows(A, lda) ? size_t(M) * aligned_cols(K) : 0;
+  return sp;
+}
 
 cudaError_t gemm(const Gemm& g, cudaStream_t s) {
   if (g.M == 0 || g.N == 0) return cudaSuccess;
@@ -113,15 +246,26 @@ cudaError_t gemm(const Gemm& g, cudaStream_t s) {
   if (!d || d->cc != 100) return cudaErrorNotSupported;
   unsigned* status = nullptr;
   if (const cudaError_t e = status::word(&status); e != cudaSuccess) return e;
-  bool tma = g.K > 0 && tma_rows(g.A, g.lda) && tma_rows(g.W, g.ldw);
-  GemmPlan p = plan_gemm(g.M, g.N, g.K, tma, d->sms);
+  const GemmPlan p = plan_gemm(g.M, g.N, g.K, d->sms);
+  // Copies of rows that TMA cannot address: the weights' first, then the tokens'.
+  Rows ra{g.A, g.lda, g.K}, rw{g.W, g.ldw, g.K};
+  const GemmSpace space = gemm_space(g.A, g.lda, g.W, g.ldw, g.M, g.N, g.K);
+  char* ws = static_cast<char*>(g.workspace);
+  if (space.w || space.a)
+    if (const cudaError_t e = align_rows(&rw, g.N, space.w ? ws : nullptr, &ra, g.M, space.a ? ws + space.w : nullptr, s);
+        e != cudaSuccess)
+      return e;
+  const bool settled = g.weights_settled && !space.w;  // a copy of the weights is not there before its kernel has ended
   CUtensorMap ta{}, tw{};
-  if (tma && (!encode_map_i8(&ta, g.A, g.K, g.M, g.lda, p.pair ? 128 : p.tile_m) ||
-              !encode_map_i8(&tw, g.W, g.K, g.N, g.ldw, 128))) {
-    tma = false;  // the driver refused the geometry
-    p = plan_gemm(g.M, g.N, g.K, false, d->sms);
-  }
-  if (p.pair) {
+  const int group = p.kernel == GemmKernel::Stream ? group_for(p.tile_m) : 1;
+  // Rows of whole k-blocks: a box may take several (one copy a stage; elsewhere
+  // the tail of a shorter last one would reach past the rows' end).
+  const bool cubes_a = group > 1 && ra.K % BK == 0, cubes_w = group > 1 && rw.K % BK == 0;
+  if (g.K > 0 && p.kernel != GemmKernel::Dot &&
+      (!encode_map_i8(&ta, ra.p, ra.K, g.M, ra.ld, p.kernel == GemmKernel::Pair ? 128 : p.tile_m, cubes_a ? group : 0) ||
+       !encode_map_i8(&tw, rw.p, rw.K, g.N, rw.ld, p.kernel == GemmKernel::Pair ? 128 : p.tile_n, cubes_w ? group : 0)))
+    return cudaErrorInvalidValue;  // the driver refused the geometry
+  if (p.kernel == GemmKernel::Pair) {
     if (p.tiles > kMaxPairUnits) return cudaErrorInvalidValue;
     PairArgs a{};
     a.u.M = g.M;
@@ -149,18 +293,36 @@ cudaError_t gemm(const Gemm& g, cudaStream_t s) {
     return launch_pair<__half>(ta, tw, a, grid, s);
   }
   if (p.grid > 0x7fffffffll) return cudaErrorInvalidValue;
+  if (p.kernel == GemmKernel::Dot) {
+    DotArgs a{};
+    a.M = g.M;
+    a.N = g.N;
+    a.K = g.K;
+    a.parts = p.splits;
+    a.weights_early = settled;
+    a.A = static_cast<const int8_t*>(ra.p);
+    a.W = static_cast<const int8_t*>(rw.p);
+    a.lda = ra.ld;
+    a.ldw = rw.ld;
+    a.ldc = g.ldc;
+    a.a_scale = g.a_scale;
+    a.w_scale = g.w_scale;
+    a.bias = g.bias;
+    a.C = g.C;
+    a.out = g.out;
+    return launch_dot(a, unsigned(p.grid), s);
+  }
   StreamArgs a{};
   a.M = g.M;
   a.N = g.N;
   a.K = g.K;
-  a.kb = ceil_div(g.K, BK);
+  a.steps = ceil_div(g.K, BK * group);
+  a.cubes_w = cubes_w;
+  a.cubes_a = cubes_a;
   a.token_tiles = ceil_div(g.M, p.tile_m);
   a.splits = p.splits;
-  a.weights_early = g.weights_settled;
-  a.A = static_cast<const int8_t*>(g.A);
-  a.W = static_cast<const int8_t*>(g.W);
-  a.lda = g.lda;
-  a.ldw = g.ldw;
+  a.weights_early = settled;
+  a.rows = p.tile_n;
   a.ldc = g.ldc;
   a.a_scale = g.a_scale;
   a.w_scale = g.w_scale;
@@ -169,8 +331,7 @@ cudaError_t gemm(const Gemm& g, cudaStream_t s) {
   a.out = g.out;
   a.status = status;
   a.wait_limit_ns = kDefaultWaitLimitNs;
-  return tma ? launch_stream<kLoadTma>(p.tile_m, tw, ta, a, unsigned(p.grid), s)
-             : launch_stream<kLoadThreads>(p.tile_m, tw, ta, a, unsigned(p.grid), s);
+  return launch_stream(p.tile_m, tw, ta, a, unsigned(p.grid), s);
 }
 
 }  // namespace aegis::i8

@@ -5,11 +5,10 @@
 // tokens cost no tensor rows and the kernel is a stream of weights.
 //
 // One CTA computes one slice of K of one 128-channel x NT-token tile:
-//   warp 0      TMA producer: a STAGES-deep ring of (weights 16 KB, tokens
-//               NT * 128 B) k-blocks;
+//   warp 0      TMA producer: a STAGES-deep ring of G k-blocks each (weights
+//               16 KB, tokens NT * 128 B a k-block);
 //   warp 1      allocates TMEM, issues the MMAs (one lane);
-//   warps 2..5  epilogue; with kLoadThreads they also fill the ring, 16 bytes
-//               at a time, for operands whose rows TMA cannot address.
+//   warps 2..5  epilogue.
 // The `splits` CTAs of a tile form one thread-block cluster. Each leaves its
 // int32 sums in its own shared memory (the ring, which is free by then), and
 // after a cluster barrier every CTA adds up an equal share of the tokens over
@@ -23,17 +22,15 @@
 
 namespace aegis::i8 {
 
-enum Load : int { kLoadTma = 0, kLoadThreads = 1 };
-
 struct StreamArgs {
   int M, N, K;
-  int kb;            // k-blocks of the whole sum
+  int steps;         // stages' worth of K (G k-blocks each) of the whole sum
+  int cubes_w, cubes_a;  // rows of whole k-blocks: the tensor map's third coordinate counts them
+  int rows;          // channels a tile: a multiple of 8, BN at most
   int token_tiles;   // tiles along the tokens (fastest in the grid, so they share weights in L2)
   int splits;        // cluster size
   int weights_early; // read weights before the grid this one depends on has completed
-  const int8_t* A;
-  const int8_t* W;
-  long long lda, ldw, ldc;
+  long long ldc;
   const float* a_scale;
   const float* w_scale;
   const void* bias;
@@ -44,12 +41,14 @@ struct StreamArgs {
 };
 
 inline constexpr int kStreamThreads = 192;
-inline constexpr int BN = 128;  // channels a tile (MMA M)
+inline constexpr int BN = 128;  // channels a tile (MMA M), at most
 
-template <int NT, int STAGES>
+template <int NT, int STAGES, int G>
 struct StreamLayout {
-  static constexpr int W_BYTES = BN * BK;
-  static constexpr int A_BYTES = NT * BK;
+  // [k-block][channel][128], `rows` channels; the MMAs read BN rows from each
+  // block's start on, the last ones of them whatever lies there, for TMEM lanes that are not stored.
+  static constexpr int W_BYTES = BN * BK * G;
+  static constexpr int A_BYTES = NT * BK * G;
   static constexpr int A_OFF = STAGES * W_BYTES;
   static constexpr int RING = STAGES * (W_BYTES + A_BYTES);
   static constexpr int BAR_OFF = RING;
@@ -62,48 +61,12 @@ struct StreamLayout {
   static_assert(NT * BN * 4 <= RING, "the int32 tile of a split fits the ring");
 };
 
-// 16 codes of a row from any byte address; bytes at or beyond `left` are zero.
-// Whole pieces are read as aligned 32-bit words (each holds at least one byte
-// of the piece) and shifted together; a row's last piece is read by bytes.
-__device__ __forceinline__ uint4 load_piece(const int8_t* p, long long left) {
-  uint32_t v[4] = {0, 0, 0, 0};
-  if (left >= 16) {
-    const uint32_t mis = uint32_t(reinterpret_cast<uintptr_t>(p) & 3u);
-    const uint32_t* q = reinterpret_cast<const uint32_t*>(p - mis);
-    uint32_t w[5];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = __ldg(q + i);
-    w[4] = mis ? __ldg(q + 4) : 0u;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = __funnelshift_r(w[i], w[i + 1], mis * 8u);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 15; ++i)
-      if (i < left) v[i >> 2] |= uint32_t(uint8_t(__ldg(p + i))) << (8 * (i & 3));
-  }
-  return make_uint4(v[0], v[1], v[2], v[3]);
-}
-
-// `rows` rows x 128 codes of a row-major matrix into a 128-byte-swizzled tile
-// at shared address `dst`, by 128 threads; rows from `limit` on and codes from
-// column K on are zero.
-__device__ __forceinline__ void fill_tile(uint32_t dst, const int8_t* base, long long ld, int row0, int rows, int limit,
-                                          int k0, int K, int tid) {
-#pragma unroll 4
-  for (int i = tid; i < rows * 8; i += 128) {
-    const int r = i >> 3, c = i & 7;
-    const int row = row0 + r, k = k0 + 16 * c;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (row < limit && k < K) v = load_piece(base + (long long)row * ld + k, K - k);
-    ptx::st_shared_v4(dst + uint32_t(r * 128 + ((c ^ (r & 7)) * 16)), v.x, v.y, v.z, v.w);
-  }
-}
-
-template <int NT, int STAGES, int LOAD>
+template <int NT, int STAGES, int G>
 __global__ void __launch_bounds__(kStreamThreads, 1)
     i8_stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmA,
                      const __grid_constant__ StreamArgs a) {
-  using L = StreamLayout<NT, STAGES>;
+  using L = StreamLayout<NT, STAGES, G>;
+  constexpr int BKS = BK * G;  // codes of K a stage
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = ptx::smem_addr(smem);
@@ -119,20 +82,23 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
   const unsigned split = blockIdx.x % unsigned(a.splits);
   const unsigned tile = blockIdx.x / unsigned(a.splits);
   const int m0 = int(tile % unsigned(a.token_tiles)) * NT;
-  const int n0 = int(tile / unsigned(a.token_tiles)) * BN;
-  const int kb0 = int((long long)a.kb * split / a.splits);
-  const int nkb = int((long long)a.kb * (split + 1) / a.splits) - kb0;
+  const int n0 = int(tile / unsigned(a.token_tiles)) * a.rows;
+  const int n_end = min(a.N, n0 + a.rows);
+  const int w_block = a.rows * BK;  // bytes of a k-block of weights
+  const uint32_t stage_bytes = uint32_t(w_block * G + L::A_BYTES);
+  const int kb0 = int((long long)a.steps * split / a.splits);  // in stages
+  const int nkb = int((long long)a.steps * (split + 1) / a.splits) - kb0;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      ptx::mbar_init(full_bar(s), LOAD == kLoadTma ? 1 : 128);
+      ptx::mbar_init(full_bar(s), 1);
       ptx::mbar_init(empty_bar(s), 1);
     }
     ptx::mbar_init(done_bar, 1);
     ptx::mbar_init(drain_bar, 1);
     *abort_flag = 0;
     ptx::fence_mbar_init();
-    if (LOAD == kLoadTma) {
+    if (nkb > 0) {
       ptx::prefetch_tensormap(&tmW);
       ptx::prefetch_tensormap(&tmA);
     }
@@ -146,25 +112,33 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
   ptx::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  int early = 0;  // k-blocks whose weights are already on their way
-  if (LOAD == kLoadTma && warp == 0 && lane == 0) {
-    const int n = min(nkb, STAGES);
-    if (a.weights_early) {
-      for (; early < n; ++early) {
-        ptx::mbar_arrive_expect_tx(full_bar(early), L::W_BYTES + L::A_BYTES);
-        ptx::tma_load_3d(sbase + early * L::W_BYTES, &tmW, full_bar(early), (kb0 + early) * BK, n0, 0);
-      }
+  // One stage's box of `rows` rows: one copy where the map counts k-blocks, else one a k-block.
+  auto copy_box = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, int step, int row0, int box_bytes, int cubes) {
+    if (cubes) {
+      ptx::tma_load_3d(dst, map, bar, 0, row0, step * G);
     } else {
-      // A hint only (ptx::tma_prefetch_3d): the copies proper follow the wait.
-      for (int i = 0; i < n; ++i)
-        if (n0 + BN <= a.N && (kb0 + i + 1) * BK <= a.K) ptx::tma_prefetch_3d(&tmW, (kb0 + i) * BK, n0, 0);
+#pragma unroll
+      for (int j = 0; j < G; ++j) ptx::tma_load_3d(dst + j * box_bytes, map, bar, (step * G + j) * BK, row0, 0);
+    }
+  };
+  int early = 0;  // stages whose weights are already on their way
+  if (warp == 0 && lane == 0) {
+    if (a.weights_early) {
+      for (const int n = min(nkb, STAGES); early < n; ++early) {
+        ptx::mbar_arrive_expect_tx(full_bar(early), stage_bytes);
+        copy_box(sbase + early * L::W_BYTES, &tmW, full_bar(early), kb0 + early, n0, w_block, a.cubes_w);
+      }
+    } else if (a.cubes_w) {
+      // Hints (ptx::tma_prefetch_3d): the copies proper follow the wait. Deeper
+      // ones, up to 64 MB in all, measured level to 20% slower.
+      for (int i = 0; i < min(nkb, STAGES); ++i) ptx::tma_prefetch_3d(&tmW, 0, n0, (kb0 + i) * G);
     }
   }
   ptx::griddep_wait();
   ptx::griddep_launch_dependents();
 
   if (warp == 0) {
-    if (LOAD == kLoadTma && lane == 0) {
+    if (lane == 0) {
       uint32_t filled = 0, fill_parity = 0;
       int stage = 0;
       uint32_t phase = 0;
@@ -174,10 +148,10 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
           if (!ptx::mbar_wait_bounded(empty_bar(stage), phase ^ 1u, abort_flag, a.status, kStatusTimeoutProducer,
                                       a.wait_limit_ns))
             break;
-          ptx::mbar_arrive_expect_tx(fb, L::W_BYTES + L::A_BYTES);
-          ptx::tma_load_3d(sbase + stage * L::W_BYTES, &tmW, fb, (kb0 + i) * BK, n0, 0);
+          ptx::mbar_arrive_expect_tx(fb, stage_bytes);
+          copy_box(sbase + stage * L::W_BYTES, &tmW, fb, kb0 + i, n0, w_block, a.cubes_w);
         }
-        ptx::tma_load_3d(sbase + L::A_OFF + stage * L::A_BYTES, &tmA, fb, (kb0 + i) * BK, m0, 0);
+        copy_box(sbase + L::A_OFF + stage * L::A_BYTES, &tmA, fb, kb0 + i, m0, NT * BK, a.cubes_a);
         filled |= 1u << stage;
         fill_parity = (fill_parity & ~(1u << stage)) | (phase << stage);
         if (++stage == STAGES) {
@@ -204,9 +178,9 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
         const uint32_t sw = sbase + stage * L::W_BYTES;
         const uint32_t sa = sbase + L::A_OFF + stage * L::A_BYTES;
 #pragma unroll
-        for (int ks = 0; ks < BK / 32; ++ks) {
-          const uint64_t wd = ptx::sdesc_sw128(sw + ks * 32u, 16u, 1024u);
-          const uint64_t ad = ptx::sdesc_sw128(sa + ks * 32u, 16u, 1024u);
+        for (int ks = 0; ks < BKS / 32; ++ks) {
+          const uint64_t wd = ptx::sdesc_sw128(sw + (ks / 4) * w_block + (ks % 4) * 32u, 16u, 1024u);
+          const uint64_t ad = ptx::sdesc_sw128(sa + (ks / 4) * (NT * BK) + (ks % 4) * 32u, 16u, 1024u);
           umma_i8(tmem_base, wd, ad, idesc, (i > 0 || ks > 0) ? 1u : 0u);
         }
         ptx::umma_commit(empty_bar(stage));
@@ -216,25 +190,6 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
         }
       }
       ptx::umma_commit(done_bar);
-    }
-    __syncwarp();
-  } else if (LOAD == kLoadThreads) {
-    const int tid = int(threadIdx.x) - 64;
-    int stage = 0;
-    uint32_t phase = 0;
-    for (int i = 0; i < nkb; ++i) {
-      if (!ptx::mbar_wait_bounded(empty_bar(stage), phase ^ 1u, abort_flag, a.status, kStatusTimeoutProducer,
-                                  a.wait_limit_ns))
-        break;
-      const int k0 = (kb0 + i) * BK;
-      fill_tile(sbase + stage * L::W_BYTES, a.W, a.ldw, n0, BN, a.N, k0, a.K, tid);
-      fill_tile(sbase + L::A_OFF + stage * L::A_BYTES, a.A, a.lda, m0, NT, a.M, k0, a.K, tid);
-      fence_proxy_async();
-      ptx::mbar_arrive(full_bar(stage));
-      if (++stage == STAGES) {
-        stage = 0;
-        phase ^= 1u;
-      }
     }
     __syncwarp();
   }
@@ -252,7 +207,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
       ptx::tc_fence_after();
     }
     const uint32_t t_row = tmem_base + (uint32_t(quarter * 32) << 16);
-    const bool live = n < a.N;
+    const bool live = n < n_end;
     const float sw = live ? __ldg(a.w_scale + n) : 0.f;
     const float b = live && a.bias ? load_as_f32(a.bias, n, a.out) : 0.f;
     constexpr int CH = NT < 32 ? NT : 32;
@@ -281,6 +236,22 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
       }
     }
   }
+  // The accumulator is read: TMEM goes back while the slices are joined. Every
+  // MMA has finished, unless the CTA gave up waiting.
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    if (*abort_flag) {
+      if (lane == 0) {
+        ptx::umma_commit(drain_bar);
+        if (!ptx::mbar_wait_teardown(drain_bar, 0, a.wait_limit_ns) && a.status)
+          atomicOr(a.status, kStatusTimeoutDrain);
+      }
+      __syncwarp();
+    }
+    ptx::tmem_dealloc(tmem_base, L::TMEM_COLS);
+  }
   if (a.splits > 1) {
     __syncwarp();
     ptx::cluster_sync();  // every slice's sums are in its CTA's shared memory
@@ -303,7 +274,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
       const int n = n0 + nl;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (n + j < a.N) {
+        if (n + j < n_end) {
           const float sw = __ldg(a.w_scale + n + j);
           const float v = a.bias ? scaled(acc[j], sa, sw, load_as_f32(a.bias, n + j, a.out)) : scaled(acc[j], sa, sw);
           store_one(a.C, (long long)(m0 + t) * a.ldc + n + j, v, a.out);
@@ -311,17 +282,6 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
     }
   }
 
-  ptx::tc_fence_before();
-  __syncthreads();
-  if (warp == 1) {
-    ptx::tc_fence_after();
-    if (lane == 0) {
-      ptx::umma_commit(drain_bar);
-      if (!ptx::mbar_wait_teardown(drain_bar, 0, a.wait_limit_ns) && a.status) atomicOr(a.status, kStatusTimeoutDrain);
-    }
-    __syncwarp();
-    ptx::tmem_dealloc(tmem_base, L::TMEM_COLS);
-  }
   if (a.splits > 1) ptx::cluster_sync();  // no CTA leaves while a peer may still read its sums
 }
 

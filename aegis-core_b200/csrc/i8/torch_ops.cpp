@@ -75,6 +75,11 @@ struct Rows {
   const void* data() const { return t.const_data_ptr(); }
 };
 
+// Torch's allocator keeps the block for later work of this stream (512-byte aligned).
+Tensor workspace(const Tensor& like, size_t bytes) {
+  return bytes ? at::empty({int64_t(bytes)}, like.options().dtype(at::kByte)) : Tensor();
+}
+
 const float* floats(const Tensor& t) { return static_cast<const float*>(t.const_data_ptr()); }
 
 Tensor matmul_i8(const Tensor& a, const Tensor& w, const Tensor& a_scale, const Tensor& w_scale,
@@ -108,8 +113,12 @@ Tensor matmul_i8(const Tensor& a, const Tensor& w, const Tensor& a_scale, const 
   const Rows ra(a), rw(w);
   const Tensor sa = a_scale.contiguous(), sw = w_scale.contiguous();
   const Tensor b = bias.defined() ? bias.contiguous() : bias;
+  size_t bytes = 0;
+  done(aegis_i8_gemm_workspace(int(M), int(N), int(K), ra.data(), ra.ld, rw.data(), rw.ld, &bytes), name);
+  const Tensor ws = workspace(a, bytes);
   done(aegis_i8_gemm(a.get_device(), stream_of(a), code, int(M), int(N), int(K), ra.data(), ra.ld, rw.data(), rw.ld,
-                     floats(sa), floats(sw), b.defined() ? b.const_data_ptr() : nullptr, out.mutable_data_ptr(), N),
+                     floats(sa), floats(sw), b.defined() ? b.const_data_ptr() : nullptr, out.mutable_data_ptr(), N,
+                     ws.defined() ? ws.mutable_data_ptr() : nullptr, bytes),
        name);
   return out;
 }
@@ -215,8 +224,8 @@ std::tuple<Tensor, Tensor> mlp_i8(const Tensor& x, const Tensor& residual, const
     const Rows rx(x), rr(residual), w1(w_gate_up), w2(w_down);
     const Tensor g = norm_weight.contiguous(), s1 = s_gate_up.contiguous(), s2 = s_down.contiguous();
     size_t bytes = 0;
-    done(aegis_i8_mlp_workspace(int(M), int(K), int(F), &bytes), name);
-    const Tensor ws = at::empty({int64_t(bytes)}, x.options().dtype(at::kByte));  // torch's allocator: 512-byte aligned
+    done(aegis_i8_mlp_workspace(int(M), int(K), int(F), w1.data(), w1.ld, w2.data(), w2.ld, &bytes), name);
+    const Tensor ws = workspace(x, bytes);
     done(aegis_i8_mlp(x.get_device(), stream_of(x), code_of(x.scalar_type()), int(M), int(K), int(F), rx.data(), rx.ld,
                       rr.data(), rr.ld, g.const_data_ptr(), float(eps), w1.data(), w1.ld, floats(s1), w2.data(), w2.ld,
                       floats(s2), h.mutable_data_ptr(), K, y.mutable_data_ptr(), K, ws.mutable_data_ptr(), bytes),

@@ -13,8 +13,10 @@ namespace aegis {
 bool encode_map(CUtensorMap* map, gemm::DType dt, const void* base, long long inner, long long outer, long long ld,
                 long long batch, long long bstride, int box_outer);
 
-// The same for rows of 8-bit codes: boxes of {128, box_outer, 1}, ld in bytes
-// (a multiple of 16, as is the base address).
-bool encode_map_i8(CUtensorMap* map, const void* base, long long inner, long long outer, long long ld, int box_outer);
+// The same for rows of 8-bit codes, ld in bytes (a multiple of 16, as is the base
+// address). blocks = 0: boxes of {128, box_outer, 1}. blocks > 0, inner a multiple
+// of 128: the rows as (128, outer, inner / 128), boxes of {128, box_outer, blocks}.
+bool encode_map_i8(CUtensorMap* map, const void* base, long long inner, long long outer, long long ld, int box_outer,
+                   int blocks = 0);
 
 }  // namespace aegis

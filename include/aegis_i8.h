@@ -19,8 +19,12 @@
  *     kernels' shared-memory limits: make that call before a stream capture.
  *     All calls may be captured into CUDA graphs after that.
  *   - Operands are device pointers of that device. Leading dimensions count
- *     elements, and every alignment is accepted. Rows whose addresses are
- *     multiples of 16 bytes are read by TMA, others by the threads.
+ *     elements, and every alignment is accepted. Rows of codes whose addresses
+ *     are multiples of 16 bytes are read as they are, others from an aligned
+ *     copy that the call makes in its workspace.
+ *   - A workspace is device memory, 256-byte aligned, of the bytes that its
+ *     query gives (0: none, NULL will do). It belongs to the call until it has
+ *     run: calls that may overlap need one each.
  *   - Outputs may not overlap inputs, unless said otherwise. Elements between
  *     the rows of an output (ld > columns) are left as they are.
  */
@@ -58,7 +62,11 @@ AEGIS_API int aegis_i8_synchronize(int device, void* stream);
  * operands or on how the work is split. */
 AEGIS_API int aegis_i8_gemm(int device, void* stream, int out_dtype, int M, int N, int K, const void* A, int64_t lda,
                             const void* W, int64_t ldw, const float* a_scale, const float* w_scale,
-                            const void* bias, void* C, int64_t ldc);
+                            const void* bias, void* C, int64_t ldc, void* workspace, size_t workspace_bytes);
+/* Bytes of workspace that call needs: 0 where the addresses of all rows of A and
+ * W are multiples of 16 bytes. Makes no CUDA call. */
+AEGIS_API int aegis_i8_gemm_workspace(int M, int N, int K, const void* A, int64_t lda, const void* W, int64_t ldw,
+                                      size_t* bytes);
 
 /* For each of `rows` rows of `cols` elements (dtype f16 or bf16):
  *   h = round(x + residual)   (residual NULL: h = x)
@@ -90,11 +98,10 @@ AEGIS_API int aegis_i8_silu_mul(int device, void* stream, int dtype, int rows, i
  *   y       = aegis_i8_gemm(q2, w_down)        [M, K] of dtype
  * with the same results as those four calls. w_gate_up: 2F x K int8, s_gate_up
  * 2F floats; w_down: K x F int8, s_down K floats. Each product starts to read
- * its weights while the row operation before it runs. The workspace (device
- * memory, 256-byte aligned, aegis_i8_mlp_workspace bytes) belongs to the call
- * until it has run: calls that may overlap need one each. M = 0: no-op.
- * K and F from 1 to AEGIS_I8_MAX_K, 2F at most 2^31 - 2^20. */
-AEGIS_API int aegis_i8_mlp_workspace(int M, int K, int F, size_t* bytes);
+ * its weights while the row operation before it runs. M = 0: no-op. K and F
+ * from 1 to AEGIS_I8_MAX_K. aegis_i8_mlp_workspace makes no CUDA call. */
+AEGIS_API int aegis_i8_mlp_workspace(int M, int K, int F, const void* w_gate_up, int64_t ld_gate_up,
+                                     const void* w_down, int64_t ld_down, size_t* bytes);
 AEGIS_API int aegis_i8_mlp(int device, void* stream, int dtype, int M, int K, int F, const void* x, int64_t ldx,
                            const void* residual, int64_t ldr, const void* norm_weight, float eps,
                            const void* w_gate_up, int64_t ld_gate_up, const float* s_gate_up, const void* w_down,
@@ -103,9 +110,8 @@ AEGIS_API int aegis_i8_mlp(int device, void* stream, int dtype, int M, int K, in
 
 /* The launch aegis_i8_gemm makes on a device with `sm_count` SMs, as JSON
  * {"kernel":..,"tile_m":..,"tile_n":..,"splits":..,"tiles":..,"grid":..}.
- * tma = 0: for operands that TMA cannot address. Needs no GPU. */
-AEGIS_API int aegis_i8_gemm_plan_json(int sm_count, int M, int N, int K, int tma, char* buf, size_t buf_len,
-                                      size_t* needed);
+ * Needs no GPU. */
+AEGIS_API int aegis_i8_gemm_plan_json(int sm_count, int M, int N, int K, char* buf, size_t buf_len, size_t* needed);
 
 #ifdef __cplusplus
 }

@@ -40,7 +40,7 @@ P = 4096  # an address that is never used: the checks come first
 
 def gemm(**kw):
     a = dict(device=0, stream=None, out_dtype=1, M=4, N=8, K=32, A=P, lda=32, W=P, ldw=32, sa=P, sw=P, bias=None,
-             C=P, ldc=8)
+             C=P, ldc=8, ws=None, wsb=0)
     a.update(kw)
     return i8.load().aegis_i8_gemm(*a.values())
 
@@ -97,25 +97,43 @@ def test_c_abi_no_ops_workspace_and_devices():
     assert gemm(M=0) == ac.AEGIS_OK and gemm(N=0, A=None, C=None) == ac.AEGIS_OK
     assert norm(rows=0, x=None) == ac.AEGIS_OK and silu(rows=0) == ac.AEGIS_OK and mlp(M=0, ws=None) == ac.AEGIS_OK
     assert mlp(ws=None) == ac.AEGIS_ERR_BUFFER_TOO_SMALL
-    assert mlp(wsb=i8.mlp_workspace(2, 32, 64) - 1) == ac.AEGIS_ERR_BUFFER_TOO_SMALL
+    assert mlp(wsb=i8.mlp_workspace(2, 32, 64, P, 32, P, 64) - 1) == ac.AEGIS_ERR_BUFFER_TOO_SMALL
     assert "workspace" in i8.last_error_string()
     assert gemm(device=-1) == ac.AEGIS_ERR_NO_DEVICE and norm(device=1 << 20) == ac.AEGIS_ERR_NO_DEVICE
     # gate_up alone takes M * 2F 16-bit values; rows of codes are padded to 16 bytes.
-    assert i8.mlp_workspace(3, 33, 65) >= 3 * (48 + 4 + 2 * 136 + 80 + 4)
-    assert i8.load().aegis_i8_mlp_workspace(1, 1, 1, None) == ac.AEGIS_ERR_INVALID_ARGUMENT
+    least = 3 * (48 + 4 + 2 * 136 + 80 + 4)
+    assert least <= i8.mlp_workspace(3, 33, 65, P, 48, P, 80) <= least + 5 * 256
+    # weights whose rows are not 16 bytes aligned are copied to rows of whole 128-code blocks
+    assert i8.mlp_workspace(3, 33, 65, P, 33, P, 80) >= least + 130 * 128
+    assert i8.mlp_workspace(3, 33, 65, P, 48, P + 1, 80) >= least + 33 * 128
+    assert i8.mlp_workspace(0, 33, 65, P, 33, P, 65) == 0
+    assert i8.load().aegis_i8_mlp_workspace(1, 1, 1, P, 1, P, 1, None) == ac.AEGIS_ERR_INVALID_ARGUMENT
     with pytest.raises(i8.AegisError):
-        i8.mlp_workspace(1, 0, 1)
+        i8.mlp_workspace(1, 0, 1, P, 16, P, 16)
+
+
+def test_product_workspace():
+    assert i8.gemm_workspace(4, 8, 32, P, 32, P, 48) == 0
+    assert i8.gemm_workspace(4, 8, 33, P, 33, P, 48) == 4 * 128
+    assert i8.gemm_workspace(4, 8, 129, P, 144, P + 8, 144) == 8 * 256
+    assert i8.gemm_workspace(4, 8, 129, P + 1, 144, P, 129) == 12 * 256
+    assert i8.gemm_workspace(4, 8, 0, P, 1, P, 1) == 0 and i8.gemm_workspace(0, 8, 33, P, 33, P, 33) == 0
+    assert i8.load().aegis_i8_gemm_workspace(-1, 8, 32, P, 32, P, 32, ctypes.byref(ctypes.c_size_t())) != ac.AEGIS_OK
+    assert i8.load().aegis_i8_gemm_workspace(4, 8, 32, P, 32, P, 32, None) == ac.AEGIS_ERR_INVALID_ARGUMENT
+    assert gemm(K=33, lda=33, ldw=48) == ac.AEGIS_ERR_BUFFER_TOO_SMALL
+    assert gemm(K=33, lda=33, ldw=48, ws=P, wsb=4 * 128 - 1) == ac.AEGIS_ERR_BUFFER_TOO_SMALL
+    assert gemm(K=33, lda=33, ldw=48, ws=P + 128, wsb=1 << 20) == ac.AEGIS_ERR_INVALID_ARGUMENT
 
 
 def test_plan_json_protocol():
     f = i8.load().aegis_i8_gemm_plan_json
     need = ctypes.c_size_t(0)
-    assert f(148, 4, 4, 4, 1, None, 0, ctypes.byref(need)) == ac.AEGIS_OK and need.value > 20
+    assert f(148, 4, 4, 4, None, 0, ctypes.byref(need)) == ac.AEGIS_OK and need.value > 20
     buf = ctypes.create_string_buffer(4)
-    assert f(148, 4, 4, 4, 1, buf, 4, None) == ac.AEGIS_ERR_BUFFER_TOO_SMALL
-    assert f(0, 4, 4, 4, 1, None, 0, None) == ac.AEGIS_ERR_INVALID_ARGUMENT
-    assert f(148, 0, 4, 4, 1, None, 0, None) == ac.AEGIS_ERR_INVALID_ARGUMENT
-    assert f(148, 4, 4, 131072, 1, None, 0, None) == ac.AEGIS_ERR_INVALID_ARGUMENT
+    assert f(148, 4, 4, 4, buf, 4, None) == ac.AEGIS_ERR_BUFFER_TOO_SMALL
+    assert f(0, 4, 4, 4, None, 0, None) == ac.AEGIS_ERR_INVALID_ARGUMENT
+    assert f(148, 0, 4, 4, None, 0, None) == ac.AEGIS_ERR_INVALID_ARGUMENT
+    assert f(148, 4, 4, 131072, None, 0, None) == ac.AEGIS_ERR_INVALID_ARGUMENT
 
 
 @pytest.mark.parametrize("sms", [1, 20, 132, 148])
@@ -123,17 +141,24 @@ def test_plans_cover_the_problem(sms):
     for M in (1, 2, 15, 16, 17, 33, 64, 100, 129, 256, 257, 1000, 8192, 100000):
         for N in (1, 64, 127, 128, 129, 4096, 14336, 151936):
             for K in (0, 1, 127, 128, 777, 4096, 131071):
-                for tma in (True, False):
-                    p = i8.gemm_plan(M, N, K, tma, sms)
-                    tiles = -(-M // p["tile_m"]) * -(-N // p["tile_n"])
-                    assert p["tiles"] == tiles
-                    if p["kernel"] == "pair":
-                        assert tma and K > 0 and p["grid"] == 2 * tiles and p["splits"] == 1
-                    else:
-                        # one CTA of a cluster a slice; at most 8 CTAs a cluster everywhere; no slice without k-blocks
-                        assert p["grid"] == tiles * p["splits"] and p["splits"] in (1, 2, 4, 8)
-                        assert p["splits"] <= max(1, -(-K // 128))
-                        assert p["tile_m"] in (16, 32, 64, 128, 256) and p["tile_n"] == 128
+                p = i8.gemm_plan(M, N, K, sms)
+                tiles = -(-M // p["tile_m"]) * -(-N // p["tile_n"])
+                assert p["tiles"] == tiles
+                if p["kernel"] == "pair":
+                    assert K > 0 and p["grid"] == 2 * tiles and p["splits"] == 1
+                elif p["kernel"] == "dot":
+                    # 8 warps a block, `splits` of them on the same channels, each with some of K
+                    assert K > 0 and M <= 8 and p["tile_m"] == M and p["splits"] in (1, 2, 4, 8)
+                    assert p["grid"] * 8 // p["splits"] >= tiles > (p["grid"] - 1) * 8 // p["splits"]
+                    assert p["splits"] == 1 or K >= 512 * p["splits"]
+                else:
+                    # one CTA of a cluster a slice; at most 8 CTAs a cluster everywhere; no slice without k-blocks
+                    assert p["grid"] == tiles * p["splits"] and p["splits"] in (1, 2, 4, 8)
+                    assert p["splits"] <= max(1, -(-K // 128))
+                    assert p["tile_m"] in (16, 32, 64, 128, 256)
+                    # whole rows of the swizzle; a cluster's slices are at most the SMs' slots
+                    assert p["tile_n"] % 8 == 0 and 8 <= p["tile_n"] <= 128
+                    assert p["splits"] == 1 or p["grid"] <= 2 * sms
 
 
 # ---------------------------------------------------------------- torch operators

@@ -140,7 +140,7 @@ def test_product_leaves_what_is_between_the_rows(ops, M, N, ldc, out):
     c = torch.full((M + 2, ldc), 7.0, device="cuda", dtype=dt)
     st = i8.load().aegis_i8_gemm(0, torch.cuda.current_stream().cuda_stream, out, M, N, 256, a.data_ptr(), 256,
                                  w.data_ptr(), 256, sa.data_ptr(), sw.data_ptr(), b.data_ptr(),
-                                 c.data_ptr() + ldc * c.element_size(), ldc)
+                                 c.data_ptr() + ldc * c.element_size(), ldc, None, 0)
     assert st == 0
     assert torch.equal(c[1:-1, :N], ops.matmul_i8(a, w, sa, sw, b, out_dtype=dt))
     c[1:-1, :N] = 7.0
