@@ -63,13 +63,13 @@ GemmPlan plan_gemm(int M, int N, int K, int sms) {
       return p;
     }
   }
-  // CTA pairs: 256 x 256 tiles, 0.36 us a k-block, and 5 more for a wave's first
-  // copies and last epilogue.
+  // CTA pairs: 256 x 256 tiles, 0.31 us a k-block, and 2.5 more for the first
+  // copies and the last epilogue.
   const long long pair_tiles = (long long)ceil_div(M, 256) * ceil_div(N, 256);
   const double dram_us = double(N) * K / 6.5e6;
   double best = 1e300;
   if (K > 0 && M > 64) {
-    best = std::max(dram_us, 5.0 + 0.36 * kb * double(ceil_div(pair_tiles, (long long)std::max(1, sms / 2))));
+    best = std::max(dram_us, 2.5 + 0.31 * kb * double(ceil_div(pair_tiles, (long long)std::max(1, sms / 2))));
     p.kernel = GemmKernel::Pair;
     p.tile_m = p.tile_n = 256;
     p.tiles = pair_tiles;
@@ -179,7 +179,7 @@ cudaError_t launch_pair(const CUtensorMap& ta, const CUtensorMap& tw, const Pair
   if (const cudaError_t e = optin.ensure(reinterpret_cast<const void*>(kern), smem); e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(umma::kThreads);
+  cfg.blockDim = dim3(kPairThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];

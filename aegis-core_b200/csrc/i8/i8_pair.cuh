@@ -8,9 +8,15 @@
 // issues M = 256, N = 256, K = 32 MMAs on both CTAs' tiles; two TMEM
 // accumulators let a tile's epilogue overlap the next one's main loop. A stage
 // has the bytes of the 16-bit kernel's (32 KB a CTA), and its MMAs take half
-// the time, so the copies have half the time to arrive. Here the epilogue
-// scales the int32 sums: a lane has one token (its scale in a register), the
-// 32 channels of a chunk share their scales across the lanes.
+// the time, so the copies have half the time to arrive.
+//
+// The epilogue matters more here: a prompt of a few hundred tokens is one tile a
+// pair, whose epilogue nothing hides. Eight warps share it, two for each 32 TMEM
+// lanes (tokens), half of the channels each; the tile's channel scales wait in
+// shared memory, the next 32 columns are on their way from TMEM while the present
+// ones are scaled and stored, 32 bytes a lane and store. With four warps, scales
+// from global memory and 16-byte stores it took 6.9 us of a 22.5 us launch
+// (256 x 14336 x 4096, B200).
 #include "../umma2_kernel.cuh"
 #include "i8_common.cuh"
 
@@ -25,48 +31,151 @@ struct PairArgs {
 };
 
 inline constexpr int kPairBN = 256, kPairStages = 7;
-using PairLayout = umma::LayoutPair<kPairBN, kPairStages>;
+inline constexpr int kPairEpilogueWarps = 8, kPairThreads = 64 + 32 * kPairEpilogueWarps;
+// umma's layout (ring, barriers, schedule), then the tile's channel scales.
+struct PairLayout : umma::LayoutPair<kPairBN, kPairStages> {
+  using Base = umma::LayoutPair<kPairBN, kPairStages>;
+  static constexpr int SCALE_OFF = (Base::BYTES + 15) / 16 * 16;
+  static constexpr int ALLOC = SCALE_OFF + kPairBN * 4 + 1024;
+  static_assert(ALLOC <= 232448, "a CTA's shared memory");
+};
 
-// 32 channels of one token: scaled, rounded, stored (ncols of them).
-template <class T>
-__device__ __forceinline__ void store_chunk(const PairArgs& a, long long row, int col, float sa, const uint32_t (&r)[32]) {
-  const int ncols = min(32, a.u.N - col);
-  float v[32];
-  if (ncols == 32 && (reinterpret_cast<uintptr_t>(a.w_scale) & 15u) == 0) {
+// Arrive on another CTA's mbarrier without waiting for this thread's stores to
+// C to be visible in the cluster (a release does: 1 us after a tile's stores). What
+// the barrier hands over is TMEM, ordered by the tcgen05 fences.
+__device__ __forceinline__ void arrive_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// Whether `v` holds for every one of `count` threads (whole warps) on hardware barrier `id`.
+__device__ __forceinline__ bool named_all(uint32_t id, uint32_t count, bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.and.pred q, %2, %3, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(uint32_t(v)), "r"(id), "r"(count)
+      : "memory");
+  return r != 0;
+}
+
+__device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
+// 32 channels of one token: scaled by sa and the scales at `scales` (shared memory),
+// plus the bias (one value a lane, for its channel).
+__device__ __forceinline__ void scale_chunk(const PairArgs& a, float sa, uint32_t scales, float bias,
+                                            const uint32_t (&r)[32], float (&v)[32]) {
 #pragma unroll
-    for (int i = 0; i < 32; i += 4) {
-      const float4 sw = __ldg(reinterpret_cast<const float4*>(a.w_scale + col + i));
-      v[i] = scaled(int(r[i]), sa, sw.x);
-      v[i + 1] = scaled(int(r[i + 1]), sa, sw.y);
-      v[i + 2] = scaled(int(r[i + 2]), sa, sw.z);
-      v[i + 3] = scaled(int(r[i + 3]), sa, sw.w);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = i < ncols ? scaled(int(r[i]), sa, __ldg(a.w_scale + col + i)) : 0.f;
+  for (int i = 0; i < 32; i += 4) {
+    const uint4 w = ptx::ld_shared_v4(scales + 4 * i);
+    v[i] = scaled(int(r[i]), sa, __uint_as_float(w.x));
+    v[i + 1] = scaled(int(r[i + 1]), sa, __uint_as_float(w.y));
+    v[i + 2] = scaled(int(r[i + 2]), sa, __uint_as_float(w.z));
+    v[i + 3] = scaled(int(r[i + 3]), sa, __uint_as_float(w.w));
   }
   if (a.bias) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (i < ncols) v[i] = __fadd_rn(v[i], load_as_f32(a.bias, col + i, a.out));
-  }
-  T* dst = static_cast<T*>(a.u.C) + row * a.u.ldc + col;
-  if constexpr (sizeof(T) == 2) {
-    umma::store_row_chunk<T>(dst, v, ncols);
-  } else {
-    if (ncols == 32 && (reinterpret_cast<uintptr_t>(dst) & 15u) == 0) {
-#pragma unroll
-      for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (i < ncols) dst[i] = v[i];
-    }
+    for (int i = 0; i < 32; ++i) v[i] = __fadd_rn(v[i], __shfl_sync(0xffffffffu, bias, i));
   }
 }
 
 template <class T>
-__global__ void __launch_bounds__(umma::kThreads, 1)
+__device__ __forceinline__ T to_out(float v) {
+  if constexpr (sizeof(T) == 2) return Elem<T>::from_f32(v);
+  else return v;
+}
+
+// A lane's row of C, 32 columns after 32. Where the row does not start on a
+// 16-byte boundary (every other row of an odd N, say) the values are shifted to
+// the boundaries in registers, the last 16 bytes of a chunk waiting for the next
+// one: single 2-byte stores, 32 rows of them an instruction, took four times the
+// whole product's time (1000 x 14331 x 4096: 190 us, the aligned N 48).
+template <class T>
+struct RowWriter {
+  static constexpr int kWords = 32 * int(sizeof(T)) / 4;  // a chunk's
+  static constexpr int kVec = 16 / int(sizeof(T));        // values in 16 bytes
+  T* at;              // the next column
+  int past;           // values since the last 16-byte boundary
+  uint32_t carry[4];  // the 16 bytes of values before `at`
+  bool begun = false;
+
+  __device__ explicit RowWriter(T* p) : at(p), past(int((reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(T))) {}
+
+  static __device__ __forceinline__ T value(const uint32_t* w, int i) {
+    if constexpr (sizeof(T) == 2) {
+      const uint16_t h = uint16_t(w[i >> 1] >> (16 * (i & 1)));
+      return reinterpret_cast<const T&>(h);
+    } else {
+      return reinterpret_cast<const T&>(w[i]);
+    }
+  }
+
+  __device__ __forceinline__ void chunk(const float (&v)[32]) {
+    uint32_t w[4 + kWords + 2];
+#pragma unroll
+    for (int j = 0; j < kWords; ++j) {
+      if constexpr (sizeof(T) == 2) w[4 + j] = Elem<T>::pack(v[2 * j], v[2 * j + 1]);
+      else w[4 + j] = __float_as_uint(v[j]);
+    }
+    if ((reinterpret_cast<uintptr_t>(at) & 31u) == 0) {
+#pragma unroll
+      for (int j = 0; j < kWords; j += 8) {
+        const uint32_t o[8] = {w[4 + j], w[5 + j], w[6 + j], w[7 + j], w[8 + j], w[9 + j], w[10 + j], w[11 + j]};
+        store32(at + j * (4 / int(sizeof(T))), o);
+      }
+    } else if (past == 0) {
+#pragma unroll
+      for (int j = 0; j < kWords; j += 4)
+        *reinterpret_cast<uint4*>(at + j * (4 / int(sizeof(T)))) = make_uint4(w[4 + j], w[5 + j], w[6 + j], w[7 + j]);
+    } else {
+      if (!begun) {  // up to the first boundary
+#pragma unroll
+        for (int i = 0; i < kVec - 1; ++i)
+          if (i < kVec - past) at[i] = value(w + 4, i);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = begun ? carry[j] : 0u;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) carry[j] = w[kWords + j];
+      w[4 + kWords] = w[5 + kWords] = 0;
+      // Values kVec - past on, of those 16 bytes and the chunk.
+      int d = kVec - past;
+      if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int j = 0; j < 4 + kWords; ++j) w[j] = d & 1 ? __funnelshift_r(w[j], w[j + 1], 16) : w[j];
+        d >>= 1;
+      }
+#pragma unroll
+      for (int j = 0; j < 4 + kWords; ++j) w[j] = d & 1 ? w[j + 1] : w[j];
+#pragma unroll
+      for (int j = 0; j < 3 + kWords; ++j) w[j] = d & 2 ? w[j + 2] : w[j];
+#pragma unroll
+      for (int j = 0; j < kWords; j += 4)
+        if (j > 0 || begun)
+          *reinterpret_cast<uint4*>(at + j * (4 / int(sizeof(T))) - past) = make_uint4(w[j], w[j + 1], w[j + 2], w[j + 3]);
+      begun = true;
+    }
+    at += 32;
+  }
+  // The values that wait for a chunk that does not come.
+  __device__ __forceinline__ void finish() {
+    if (begun) {
+#pragma unroll
+      for (int i = 1; i < kVec; ++i)
+        if (i >= kVec - past) at[i - kVec] = value(carry, i);
+    }
+    begun = false;
+  }
+};
+
+template <class T>
+__global__ void __launch_bounds__(kPairThreads, 1)
     i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
                    const __grid_constant__ PairArgs p) {
   using L = PairLayout;
@@ -98,22 +207,16 @@ __global__ void __launch_bounds__(umma::kThreads, 1)
     }
     for (int acc = 0; acc < 2; ++acc) {
       ptx::mbar_init(tfull_bar(acc), 1);
-      ptx::mbar_init(tempty_bar(acc), 256);  // every epilogue thread of both CTAs
+      ptx::mbar_init(tempty_bar(acc), 2 * kPairEpilogueWarps);  // one lane a warp, both CTAs
     }
     ptx::mbar_init(drain_bar, 1);
-    sched.init(10);  // 1 + 4 readers in the leader, 1 + 4 in the peer
+    sched.init(2 * (1 + kPairEpilogueWarps));  // readers: MMA lane and epilogue warps; peer's producer and its
     *abort_flag = 0;
     ptx::fence_mbar_init();
   }
   if (warp == 0 && lane == 0) {
     ptx::prefetch_tensormap(&tmA);
     ptx::prefetch_tensormap(&tmW);
-    // The weights of the first k-blocks into L2 while the previous grid ends
-    // (a hint, see ptx::tma_prefetch_3d); the tokens are often its output.
-    const Unit u = umma::decode_unit_pair<kPairBN>(a, first_unit);
-    const int wn = u.n0 + 128 * int(rank);
-    for (int i = 0; i < min(u.nkb, STAGES); ++i)
-      if (wn + 128 <= a.N && (i + 1) * BK <= a.K) ptx::tma_prefetch_3d(&tmW, i * BK, wn, 0);
   }
   if (warp == 1) {
     ptx::tmem_alloc_pair(ptx::smem_addr(tmem_slot), L::TMEM_COLS);
@@ -213,9 +316,12 @@ __global__ void __launch_bounds__(umma::kThreads, 1)
       __syncwarp();
     }
   } else {
-    // ------------------------------------------------ epilogue (warps 2..5, both CTAs)
-    const int quarter = warp & 3;
+    // ------------------------------------------------ epilogue (warps 2..9, both CTAs)
+    constexpr int kHalf = kPairBN / 2;
+    const int quarter = warp & 3, first = ((warp - 2) >> 2) * kHalf;  // TMEM lanes, first column
+    const int et = int(threadIdx.x) - 64;                            // 0..255: the column whose scale it fetches
     const int row_in_tile = 128 * int(rank) + quarter * 32 + lane;
+    const uint32_t scales = sbase + L::SCALE_OFF;
     int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
@@ -223,27 +329,59 @@ __global__ void __launch_bounds__(umma::kThreads, 1)
     for (long long unit = first_unit; ok && unit >= 0;) {
       const Unit u = umma::decode_unit_pair<kPairBN>(a, unit);
       const int row = u.m0 + row_in_tile;
-      const float sa = row < a.M ? __ldg(p.a_scale + row) : 0.f;
+      const bool live = row < a.M;
+      const float sa = live ? __ldg(p.a_scale + row) : 0.f;
+      const float sw = u.n0 + et < a.N ? __ldg(p.w_scale + u.n0 + et) : 0.f;
+      float bias[kHalf / 32];
+#pragma unroll
+      for (int c = 0; c < kHalf / 32; ++c) {
+        const int col = u.n0 + first + 32 * c + lane;
+        bias[c] = p.bias && col < a.N ? load_as_f32(p.bias, col, p.out) : 0.f;
+      }
+      ptx::named_barrier(1, 32 * kPairEpilogueWarps);  // the last tile's scales are read
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(scales + 4u * uint32_t(et)), "f"(sw) : "memory");
+      ptx::named_barrier(1, 32 * kPairEpilogueWarps);
       if (lane == 0)
         ok = ptx::mbar_wait_bounded(tfull_bar(acc), acc_phase, abort_flag, a.status, kStatusTimeoutEpilogue,
                                     a.wait_limit_ns);
-      ok = __shfl_sync(0xffffffffu, ok, 0);
+      // One answer for all eight warps: a warp that left alone would strand the others at the barriers.
+      ok = named_all(2, 32 * kPairEpilogueWarps, __shfl_sync(0xffffffffu, ok, 0));
       if (!ok) break;
       ptx::tc_fence_after();
-      const uint32_t t_row = tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(acc * kPairBN);
-      for (int c = 0; c < kPairBN && u.n0 + c < a.N; c += 32) {
-        uint32_t r[32];
-        ptx::tmem_ld_32x32b_x32(t_row + c, r);
-        ptx::tmem_ld_wait(r);
-        if (row < a.M) store_chunk<T>(p, row, u.n0 + c, sa, r);
+      const uint32_t t_row = tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(acc * kPairBN + first);
+      RowWriter<T> out(static_cast<T*>(a.C) + (live ? row : 0) * a.ldc + u.n0 + first);
+      uint32_t r[2][32];
+      ptx::tmem_ld_32x32b_x32(t_row, r[0]);
+#pragma unroll
+      for (int c = 0; c < kHalf / 32; ++c) {
+        ptx::tmem_ld_wait(r[c & 1]);
+        if (c + 1 < kHalf / 32) {
+          ptx::tmem_ld_32x32b_x32(t_row + 32 * (c + 1), r[(c + 1) & 1]);
+        } else {
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_relaxed(ptx::map_to_rank(tempty_bar(acc), 0));  // the accumulator is read
+        }
+        const int col = u.n0 + first + 32 * c;
+        if (col >= a.N) continue;
+        float v[32];
+        scale_chunk(p, sa, scales + 4u * uint32_t(first + 32 * c), bias[c], r[c & 1], v);
+        if (!live) continue;
+        if (col + 32 <= a.N) {
+          out.chunk(v);
+        } else {
+          out.finish();
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (col + i < a.N) out.at[i] = to_out<T>(v[i]);
+        }
       }
-      ptx::tc_fence_before();
-      ptx::mbar_arrive_cluster(ptx::map_to_rank(tempty_bar(acc), 0));
+      if (live) out.finish();
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1u;
       long long next = -1;
       if (lane == 0) ok = umma::sched_take(sched, seq, rank != 0, &next, kStatusTimeoutEpilogue);
-      ok = __shfl_sync(0xffffffffu, ok, 0);
+      ok = named_all(2, 32 * kPairEpilogueWarps, __shfl_sync(0xffffffffu, ok, 0));
       unit = __shfl_sync(0xffffffffu, next, 0);
     }
   }

@@ -171,6 +171,28 @@ def test_strides_of_every_kind(ops):
     assert torch.equal(q, q2) and torch.equal(s, s2) and torch.equal(h, h2)
 
 
+@pytest.mark.parametrize("M,N,ldc,offset", [(1100, 4099, 4099, 0), (1100, 4099, 4100, 3), (1030, 6401, 6403, 1),
+                                            (1100, 4099, 4101, 5), (1100, 4352, 4353, 7), (1100, 4352, 4368, 8),
+                                            (1300, 4133, 4144, 0), (1030, 6401, 6402, 2)])
+@pytest.mark.parametrize("out", ["float16", "bfloat16", "float32"])
+@pytest.mark.parametrize("bias", [True, False])
+def test_large_products_into_rows_of_any_alignment(ops, M, N, ldc, offset, out, bias):
+    import torch
+    import aegis_i8 as i8
+    assert i8.gemm_plan(M, N, 512)["kernel"] == "pair"
+    dt = getattr(torch, out)
+    a, w, sa, sw, b = make(torch, M + N, M, N, 512, 0, 0, dt if bias else None)
+    buf = torch.full((offset + (M + 1) * ldc,), 7.0, device="cuda", dtype=dt)
+    st = i8.load().aegis_i8_gemm(0, torch.cuda.current_stream().cuda_stream, {"float16": 0, "bfloat16": 1, "float32": 2}[out],
+                                 M, N, 512, a.data_ptr(), 512, w.data_ptr(), 512, sa.data_ptr(), sw.data_ptr(),
+                                 b.data_ptr() if bias else None, buf.data_ptr() + offset * buf.element_size(), ldc, None, 0)
+    assert st == 0
+    c = buf[offset:].view(M + 1, ldc)
+    assert_product(torch, c[:M, :N], a, w, sa, sw, b)
+    c[:M, :N] = 7.0
+    assert (buf == 7.0).all()
+
+
 def test_product_scales_that_are_not_finite(ops):
     import torch
     a, w, sa, sw, _ = make(torch, 9, 20, 40, 128)
