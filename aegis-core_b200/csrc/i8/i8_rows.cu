@@ -303,37 +303,42 @@ __device__ __noinline__ double block_reduce64(double v, bool sum, double* buf) {
   return v;
 }
 
-// The code of column c in 64 bits. Out of line: one copy for the few elements at a border.
+// The code of column c in 64 bits.
 template <class T, int MODE>
-__device__ __noinline__ int code64(Row<T, MODE> row, int c, double m64) {
+__device__ __forceinline__ int code64(const Row<T, MODE>& row, int c, double m64) {
   return int(rint(127.0 * row.t64(c) / m64));
 }
 template <class T, int MODE>
-__device__ __noinline__ double abs_t64(Row<T, MODE> row, int c) {
+__device__ __forceinline__ double abs_t64(const Row<T, MODE>& row, int c) {
   return fabs(row.t64(c));
 }
 
-// The sum of the row's squares in double, for rows whose squares leave float's range.
+// A whole row in double: rows of zeros, rows that are not finite, and those for
+// which float's range or precision does not do. Each thread reads the columns whose h
+// it stored itself. Out of line, and called where nothing else is alive.
 template <class T, int MODE>
-__device__ __noinline__ double squares64(Row<T, MODE> row, int cols, double* buf) {
-  double s = 0.0;
-  for (int c0 = int(threadIdx.x) * 8; c0 < cols; c0 += int(blockDim.x) * 8)
-    for (int c = c0; c < min(c0 + 8, cols); ++c) s += row.norm_input(c) * row.norm_input(c);
-  return block_reduce64(s, true, buf);
-}
-
-// A row of zeros, or of numbers for which float's range or precision does not
-// do, all in double. Each thread reads the columns whose h it stored itself.
-// Returns the row's maximum.
-template <class T, int MODE>
-__device__ __noinline__ double row_in_double(Row<T, MODE> row, int cols, int8_t* q, double* buf) {
-  double m = 0.0;
-  for (int c0 = int(threadIdx.x) * 8; c0 < cols; c0 += int(blockDim.x) * 8)
-    for (int c = c0; c < min(c0 + 8, cols); ++c) m = max_nan(fabs(row.t64(c)), m);
+__device__ __noinline__ void row_in_double(const RowArgs& a, int ri, double* buf) {
+  const Row<T, MODE> row(a, ri);
+  int8_t* q = a.q + (long long)ri * a.ldq;
+  const int cols = a.cols, step = int(blockDim.x) * 8;
+  double m = 0.0, s = 0.0;
+  for (int c0 = int(threadIdx.x) * 8; c0 < cols; c0 += step)
+    for (int c = c0; c < min(c0 + 8, cols); ++c) {
+      m = max_nan(fabs(row.t64(c)), m);
+      if (MODE != kSilu) s += row.norm_input(c) * row.norm_input(c);
+    }
   m = block_reduce64(m, false, buf);
-  for (int c0 = int(threadIdx.x) * 8; c0 < cols; c0 += int(blockDim.x) * 8)
-    for (int c = c0; c < min(c0 + 8, cols); ++c) q[c] = m > 0.0 && m <= kMost ? int8_t(code64<T, MODE>(row, c, m)) : int8_t(0);
-  return m;
+  if (MODE != kSilu) s = block_reduce64(s, true, buf);
+  // t is finite in 32 bits, and so is h (an infinite h gives an infinite t, or NaN where the weight is 0).
+  const bool fine = m <= kMost;
+  for (int c0 = int(threadIdx.x) * 8; c0 < cols; c0 += step)
+    for (int c = c0; c < min(c0 + 8, cols); ++c)
+      q[c] = fine && m > 0.0 ? int8_t(code64<T, MODE>(row, c, m)) : int8_t(0);
+  if (threadIdx.x == 0) {
+    float scale = float(m / 127.0);
+    if (MODE != kSilu) scale = m > 0.0 ? float(m / (127.0 * sqrt(s / cols + double(a.eps)))) : 0.f;
+    a.scale[ri] = fine ? scale : __int_as_float(0x7fc00000);
+  }
 }
 
 __device__ __forceinline__ float at(const f32x2 (&t)[4], int i) {
@@ -384,87 +389,81 @@ __device__ __forceinline__ void copy_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// What the two kernels below share: the row's maximum in 64 bits, its scale, and what
-// silu leaves to do until the next row's barrier.
-template <class T, int MODE>
-struct Finish {
+// Whether a row has to be taken in double: `gates` (silu, any thread's), a largest
+// magnitude that is tiny or not finite, squares that left float's range.
+template <int MODE>
+__device__ __forceinline__ bool needs_double(const Found& f, int gates) {
+  const bool m = !(f.m >= kTiny && f.m <= 3.4028235e38f);
+  return MODE == kSilu ? m || gates : m || !(f.ss < 1e37f) || f.ss < 1e-25f;
+}
+
+__device__ __forceinline__ float norm_scale(const RowArgs& a, const Found& f) {
+  return f.m / (127.f * sqrtf(f.ss / float(a.cols) + a.eps));
+}
+
+// What a silu row leaves to do until the next row's barrier.
+template <class T>
+struct Behind {
   const RowArgs& a;
   unsigned long long* top64;  // row maxima in 64 bits, of three rows in turn: the bits
                               // of a double that is not negative order as it does
-  double* buf64;
-  uint32_t border_bits = 0;   // elements of row `behind` at a border (silu)
-  int behind = -1;
+  uint32_t border_bits = 0;   // elements of row `row` at a border
+  int row = -1;
   unsigned slot = 0;          // its place in top64
-  unsigned turn = 0;          // this row's: 0, 1, 2, 0, ...
-  double m64 = 0.0;
+  unsigned turn = 0;          // the present row's: 0, 1, 2, 0, ...
 
   __device__ int column(int i) const {  // of the thread's i-th element
     return ((i >> 3) * int(blockDim.x) + int(threadIdx.x)) * 8 + (i & 7);
   }
-  __device__ void set_codes(int ri, uint32_t bits, double top) const {
-    const Row<T, MODE> row(a, ri);
-    for (; bits; bits &= bits - 1) {
-      const int c = column(__ffs(int(bits)) - 1);
-      if (c < a.cols) a.q[(long long)ri * a.ldq + c] = int8_t(code64<T, MODE>(row, c, top));
-    }
+  // After the present row's barrier: the next row's slot (its last readers are past the barrier).
+  __device__ void begin() {
+    if (threadIdx.x == 0) top64[turn == 2 ? 0 : turn + 1] = 0;
   }
-  // Silu, between the barriers of the next row and the one after it (or behind
-  // a barrier of its own). Where it is called, t is no longer needed: t kept over the
-  // calls in here cost 34 registers' spills a row.
-  __device__ void settle() {
-    if (MODE != kSilu || behind < 0) return;
-    const double top = __longlong_as_double((long long)top64[slot]);
-    if (threadIdx.x == 0) a.scale[behind] = float(top / 127.0);
-    if (border_bits) set_codes(behind, border_bits, top);
-    border_bits = 0;
-    behind = -1;
-  }
-  // Right after row ri's barrier. True: the row is done (not finite, or in double).
-  __device__ bool begin(int ri, const Found& f, int in_double) {
-    if (MODE == kSilu && threadIdx.x == 0) top64[turn == 2 ? 0 : turn + 1] = 0;  // the next row's; its readers are past the barrier
-    in_double |= f.m < kTiny;
-    m64 = double(f.m);
-    if (!in_double && f.m <= 3.4028235e38f) return false;
-    const Row<T, MODE> row(a, ri);
-    int8_t* q = a.q + (long long)ri * a.ldq;
-    if (in_double) m64 = row_in_double<T, MODE>(row, a.cols, q, buf64);
-    if (!(m64 <= kMost)) {
-      // Not finite: codes 0, scale NaN. (An infinite h gives a t that is infinite, or NaN where the weight is 0.)
-      for (int c0 = int(threadIdx.x) * 8; c0 < a.cols; c0 += int(blockDim.x) * 8)
-        for (int c = c0; c < min(c0 + 8, a.cols); ++c) q[c] = 0;
-      if (threadIdx.x == 0) a.scale[ri] = __int_as_float(0x7fc00000);
-    } else if (MODE == kSilu) {
-      if (threadIdx.x == 0) a.scale[ri] = float(m64 / 127.0);
-    } else {
-      norm_scale(ri, f);
-    }
-    return true;
-  }
-  __device__ void norm_scale(int ri, const Found& f) const {
-    if (!(f.ss < 1e37f) || f.ss < 1e-25f) {  // squares that left float's range are summed again in double
-      const double sum = squares64<T, MODE>(Row<T, MODE>(a, ri), a.cols, buf64);
-      if (threadIdx.x == 0)
-        a.scale[ri] = m64 > 0.0 ? float(m64 / (127.0 * sqrt(sum / a.cols + double(a.eps)))) : 0.f;
-    } else if (threadIdx.x == 0) {
-      a.scale[ri] = float(m64) / (127.f * sqrtf(f.ss / float(a.cols) + a.eps));
-    }
-  }
-  // Silu: element i of this thread can be the row's maximum.
+  // Element i of this thread can be row ri's maximum.
   __device__ void candidate(int ri, int i) const {
-    const double d = abs_t64<T, MODE>(Row<T, MODE>(a, ri), column(i));
+    const double d = abs_t64<T, kSilu>(Row<T, kSilu>(a, ri), column(i));
     atomicMax(&top64[turn], (unsigned long long)__double_as_longlong(d));
+  }
+  // Between the barriers of the next row and the one after it (or behind a barrier
+  // of its own). Where this is called, t is no longer needed: kept over what is in
+  // here it cost a third of the registers.
+  __device__ void settle() {
+    if (row < 0) return;
+    const double top = __longlong_as_double((long long)top64[slot]);
+    if (threadIdx.x == 0) a.scale[row] = float(top / 127.0);
+    if (border_bits) {
+      const Row<T, kSilu> r(a, row);
+      for (; border_bits; border_bits &= border_bits - 1) {
+        const int c = column(__ffs(int(border_bits)) - 1);
+        if (c < a.cols) a.q[(long long)row * a.ldq + c] = int8_t(code64<T, kSilu>(r, c, top));
+      }
+    }
+    row = -1;
   }
   // The end of row ri: settles the row before, and leaves `bits` of this one for later (done: nothing).
   __device__ void end(int ri, uint32_t bits, bool done) {
     settle();
     if (!done) {
       border_bits = bits;
-      behind = ri;
+      row = ri;
       slot = turn;
     }
     turn = turn == 2 ? 0 : turn + 1;
   }
 };
+
+// Elements of a norm row at a border, a bit each of this thread's.
+template <class T, int MODE>
+__device__ __forceinline__ void set_codes(const RowArgs& a, int ri, uint32_t bits, float m) {
+  const Row<T, MODE> row(a, ri);
+  for (; bits; bits &= bits - 1) {
+    const int i = __ffs(int(bits)) - 1;
+    const int c = ((i >> 3) * int(blockDim.x) + int(threadIdx.x)) * 8 + (i & 7);
+    if (c < a.cols) a.q[(long long)ri * a.ldq + c] = int8_t(code64<T, MODE>(row, c, double(m)));
+  }
+}
+
+constexpr unsigned kLater = 0x7fc00001;  // a NaN no kernel gives: marks the scale of a row that is still to be done
 
 // Many rows. Blocks of as many threads as a row of 32 elements a thread takes;
 // every row starts on a 16-byte boundary (q's on 8) and has whole pieces.
@@ -501,7 +500,8 @@ __global__ void __launch_bounds__(MOST, BLOCKS) i8_rows_kernel(const __grid_cons
     if (v < pieces) copy_piece(v);
   copy_commit();
 
-  Finish<T, MODE> fin{a, top64, buf64};
+  Behind<T> behind{a, top64};
+  bool later = false;
   unsigned par = 0;
   for (int ri = int(blockIdx.x);; par ^= 1u) {
     const bool more = a.rows - ri > rows_ahead;
@@ -525,9 +525,13 @@ __global__ void __launch_bounds__(MOST, BLOCKS) i8_rows_kernel(const __grid_cons
     const int in_double = MODE == kSilu && (st.gate() > kMostGate || (Elem<T>::kBf16 && st.most_up() > kMostUp));
     int any = in_double;
     const Found f = block_find<MODE>(st.m, both(st.ss).x + both(st.ss).y, st.gate(), &any, buf[par]);
-    const bool done = fin.begin(ri, f, any);
+    if (MODE == kSilu) behind.begin();
+    const bool done = needs_double<MODE>(f, any);
     uint32_t near = 0, can = 0;
-    if (!done) {
+    if (done) {
+      later = true;
+      if (tid == 0) a.scale[ri] = __uint_as_float(kLater);
+    } else {
       const float inv = 127.f / f.m;
       const float border = MODE == kSilu ? border_silu(f.gate) : kBorderNorm;
       float most = 0.f;
@@ -548,13 +552,13 @@ __global__ void __launch_bounds__(MOST, BLOCKS) i8_rows_kernel(const __grid_cons
 #pragma unroll
             for (int i = 0; i < 8; ++i) can |= fabsf(at(t[v], i)) >= least ? 1u << (8 * v + i) : 0u;
       }
-      if (MODE != kSilu) fin.norm_scale(ri, f);
+      if (MODE != kSilu && tid == 0) a.scale[ri] = norm_scale(a, f);
     }
     if constexpr (MODE == kSilu) {
-      for (; can; can &= can - 1) fin.candidate(ri, __ffs(int(can)) - 1);
-      fin.end(ri, near, done);
+      for (; can; can &= can - 1) behind.candidate(ri, __ffs(int(can)) - 1);
+      behind.end(ri, near, done);
     } else if (near) {
-      fin.set_codes(ri, near, fin.m64);
+      set_codes<T, MODE>(a, ri, near, f.m);
     }
     if (!more) break;
     ri += rows_ahead;
@@ -563,7 +567,14 @@ __global__ void __launch_bounds__(MOST, BLOCKS) i8_rows_kernel(const __grid_cons
   }
   if constexpr (MODE == kSilu) {
     __syncthreads();
-    fin.settle();
+    behind.settle();
+  }
+  if (later) {  // the same for all threads
+    __syncthreads();
+    for (int ri = int(blockIdx.x);; ri += rows_ahead) {
+      if (__float_as_uint(*const_cast<volatile float*>(a.scale + ri)) == kLater) row_in_double<T, MODE>(a, ri, buf64);
+      if (a.rows - ri <= rows_ahead) break;
+    }
   }
 }
 
@@ -593,14 +604,18 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) i8_row_kernel(const _
   }
   int any = MODE == kSilu && (st.gate() > kMostGate || st.most_up() > kMostUp);
   const Found f = block_find<MODE>(st.m, both(st.ss).x + both(st.ss).y, st.gate(), &any, buf);
-  Finish<T, MODE> fin{a, top64, buf64};
-  if (fin.begin(ri, f, any)) return;
+  if (needs_double<MODE>(f, any)) {
+    row_in_double<T, MODE>(a, ri, buf64);
+    return;
+  }
+  Behind<T> behind{a, top64};
   const float inv = 127.f / f.m;
   const float border = MODE == kSilu ? border_silu(f.gate) : kBorderNorm;
   const float least = f.m * near_max(f.gate);
+  if (MODE != kSilu && tid == 0) a.scale[ri] = norm_scale(a, f);
   if constexpr (VPT > 0) {
     float most = 0.f;
-    uint32_t near = 0;
+    uint32_t near = 0, can = 0;
 #pragma unroll
     for (int v = 0; v < VPT; ++v)
       if (piece(v) < a.cols)
@@ -612,37 +627,33 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) i8_row_kernel(const _
     }
     if constexpr (MODE == kSilu) {
       if (st.m >= least) {
-        uint32_t can = 0;
 #pragma unroll
         for (int v = 0; v < VPT; ++v)
           if (piece(v) < a.cols)
 #pragma unroll
             for (int i = 0; i < 8; ++i) can |= fabsf(at(t[v], i)) >= least ? 1u << (8 * v + i) : 0u;
-        for (; can; can &= can - 1) fin.candidate(ri, __ffs(int(can)) - 1);
+        for (; can; can &= can - 1) behind.candidate(ri, __ffs(int(can)) - 1);
       }
-      fin.end(ri, near, false);
+      behind.end(ri, near, false);
       __syncthreads();
-      fin.settle();
-    } else {
-      if (near) fin.set_codes(ri, near, fin.m64);
-      fin.norm_scale(ri, f);
+      behind.settle();
+    } else if (near) {
+      set_codes<T, MODE>(a, ri, near, f.m);
     }
   } else {
-    double m64 = fin.m64;
+    double m64 = double(f.m);
     if constexpr (MODE == kSilu) {
       for (int v = 0; piece(v) < a.cols; ++v) {
         Stats<T> unused;
         load_eval8<T, MODE>(a, row, piece(v), t[0], unused);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (fabsf(at(t[0], i)) >= least) fin.candidate(ri, 8 * v + i);
+          if (fabsf(at(t[0], i)) >= least) behind.candidate(ri, 8 * v + i);
       }
-      fin.end(ri, 0, false);
+      behind.end(ri, 0, false);
       __syncthreads();
+      behind.settle();
       m64 = __longlong_as_double((long long)top64[0]);  // the first row's slot
-      fin.settle();
-    } else {
-      fin.norm_scale(ri, f);
     }
     for (int v = 0; piece(v) < a.cols; ++v) {
       const int c = piece(v);
@@ -659,8 +670,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) i8_row_kernel(const _
       store_codes(q, c, a.cols, a.vec_q, quantise8(t[0], inv, border, most));
       if (most > first_test(border))
         for (uint32_t b = near_border(t[0], inv, border); b; b &= b - 1) {
-          const int at = c + __ffs(int(b)) - 1;
-          if (at < a.cols) q[at] = int8_t(code64<T, MODE>(row, at, m64));
+          const int k = c + __ffs(int(b)) - 1;
+          if (k < a.cols) q[k] = int8_t(code64<T, MODE>(row, k, m64));
         }
     }
   }
