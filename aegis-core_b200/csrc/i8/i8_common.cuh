@@ -39,6 +39,13 @@ __device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t a_desc, u
 // Makes this thread's shared-memory stores visible to the tensor core's reads.
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// Barrier of the cluster's threads that only keeps its CTAs in step: no CTA leaves
+// before the others have read its shared memory. cluster_sync's release would also
+// wait for this thread's stores to C to be visible (0.7 us).
+__device__ __forceinline__ void cluster_step() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+
 // 16 bytes of another CTA's shared memory (a shared::cluster address).
 __device__ __forceinline__ int4 ld_cluster_v4(uint32_t cluster_addr) {
   int4 v;

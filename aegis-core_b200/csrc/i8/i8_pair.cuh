@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             phase ^= 1u;
           }
         }
-        if (!ok) break;
+        if (!ok || !a.steal) break;  // one tile a pair: no schedule
         ok = rank == 0 ? owner.publish_next(sched, 2, true, &unit, kStatusTimeoutProducer)
                        : umma::sched_take(sched, seq, true, &unit, kStatusTimeoutProducer);
       }
@@ -310,6 +310,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           ptx::umma_commit_pair(tfull_bar(acc), 0x3);
           acc ^= 1;
           if (acc == 0) acc_phase ^= 1u;
+          if (!a.steal) break;
           ok = umma::sched_take(sched, seq, false, &unit, kStatusTimeoutMma);
         }
       }
@@ -379,6 +380,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       if (live) out.finish();
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1u;
+      if (!a.steal) break;
       long long next = -1;
       if (lane == 0) ok = umma::sched_take(sched, seq, rank != 0, &next, kStatusTimeoutEpilogue);
       ok = named_all(2, 32 * kPairEpilogueWarps, __shfl_sync(0xffffffffu, ok, 0));
@@ -395,7 +397,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   }
   __syncwarp();
   ptx::tc_fence_before();
-  ptx::cluster_sync();
+  cluster_step();  // neither CTA leaves while its peer may still touch its memory
   ptx::tc_fence_after();
   if (warp == 1) ptx::tmem_dealloc_pair(tmem_base, L::TMEM_COLS);
 }

@@ -282,7 +282,10 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
     }
   }
 
-  if (a.splits > 1) ptx::cluster_sync();  // no CTA leaves while a peer may still read its sums
+  if (a.splits > 1) {
+    __syncwarp();
+    cluster_step();  // no CTA leaves while a peer may still read its sums
+  }
 }
 
 }  // namespace aegis::i8
