@@ -25,7 +25,8 @@ def ops(request):
     if not torch.cuda.is_available():
         pytest.skip("no CUDA device")
     import aegis_torch  # noqa: F401
-    return torch.ops.aegis
+    yield torch.ops.aegis
+    torch.cuda.empty_cache()  # the largest tests take some 15 GB
 
 
 def gen(torch, seed):
@@ -363,6 +364,56 @@ def test_norm_in_place(ops, cols, place):
     assert st == 0
     assert torch.equal(q[:, :cols], q0) and torch.equal(s, s0) and torch.equal(h[:, :cols], h0)
     assert (q[:, cols:] == 99).all() and torch.equal(h[:, cols:], edge)
+
+
+# ---------------------------------------------------------------- offsets beyond 32 bits
+def test_product_with_an_output_beyond_2_31_elements(ops):
+    import torch
+    M, N, K = 70001, 32771, 48
+    a, w, sa, sw, _ = make(torch, 31, M, N, K)
+    c = ops.matmul_i8(a, w, sa, sw)
+    rows = torch.tensor([0, 1, 32768, 65535, 65537, M - 2, M - 1], device="cuda")
+    assert_product(torch, c[rows], a[rows], w, sa[rows], sw)
+    cols = torch.tensor([0, 32767, N - 1], device="cuda")
+    assert_product(torch, c[:, cols], a, w[cols], sa, sw[cols])
+
+
+@pytest.mark.parametrize("cols", [16392, 16391])
+def test_rows_beyond_2_31_elements(ops, cols):
+    import torch
+    rows = 140000
+    g = gen(torch, cols)
+    x = torch.empty(rows, cols, device="cuda", dtype=torch.bfloat16)
+    x[:1000] = torch.randn(1000, cols, device="cuda", generator=g).bfloat16()
+    for i in range(1000, rows, 1000):
+        x[i:i + 1000] = x[:1000]
+    w = (torch.randn(cols, device="cuda", generator=g) + 1).bfloat16()
+    pick = torch.tensor([0, 999, 131000, 131072, rows - 1], device="cuda")
+    q, s, h = ops.add_rmsnorm_i8(x, x, w, 1e-5)
+    assert torch.equal(h[pick], x[pick] * 2)
+    check_norm(torch, q[pick], s[pick], h[pick], w, 1e-5)
+    assert torch.equal(q[rows - 1000:], q[:1000]) and torch.equal(s[rows - 1000:], s[:1000])
+    del q, s, h
+    q, s = ops.silu_mul_i8(x, x)
+    xd = x[pick].double()
+    check_codes(torch, q[pick], xd / (1 + torch.exp(-xd)) * xd)
+    assert torch.equal(q[rows - 1000:], q[:1000])
+
+
+def test_codes_of_a_matrix_beyond_2_31_bytes(ops):
+    import torch
+    K, N = 4096, 530001
+    w = torch.empty(N, K, device="cuda", dtype=torch.int8)
+    w[:1000] = torch.randint(-128, 128, (1000, K), device="cuda", generator=gen(torch, 3), dtype=torch.int8)
+    for i in range(1000, N, 1000):
+        w[i:i + 1000] = w[:min(1000, N - i)]
+    sw = torch.rand(N, device="cuda") * 0.01 + 1e-3
+    pick = torch.tensor([0, 524287, 524288, N - 1], device="cuda")
+    for M in (1, 16):
+        a, _, sa, _, _ = make(torch, M, M, 8, K)
+        assert_product(torch, ops.matmul_i8(a, w, sa, sw)[:, pick], a, w[pick], sa, sw[pick])
+    a, _, sa, _, _ = make(torch, 5, 3, 8, K - 1)
+    assert_product(torch, ops.matmul_i8(a, w[:, 1:], sa, sw)[:, pick], a, w[pick, 1:], sa, sw[pick])
 
 
 # ---------------------------------------------------------------- the block
