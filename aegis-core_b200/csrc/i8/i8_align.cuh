@@ -50,8 +50,8 @@ __global__ void __launch_bounds__(kAlignThreads) i8_align_kernel(const __grid_co
     lo[u] = hi[u] = 0;
     // Words that lie inside the row; those across its ends are put together below.
     const uint32_t* q = reinterpret_cast<const uint32_t*>(src + k - mis);
-    if (k >= mis && k - mis + 4 <= a.K) lo[u] = __ldg(q);
-    if (mis != 0 && k - mis + 8 <= a.K) hi[u] = __ldg(q + 1);
+    if (k >= mis && k - mis + 4 <= a.K) lo[u] = *q;
+    if (mis != 0 && k - mis + 8 <= a.K) hi[u] = q[1];
   }
 #pragma unroll
   for (int u = 0; u < kAlignWords; ++u) {
@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(kAlignThreads) i8_align_kernel(const __grid_co
       v = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (k + i < a.K) v |= uint32_t(uint8_t(__ldg(src + k + i))) << (8 * i);
+        if (k + i < a.K) v |= uint32_t(uint8_t(src[k + i])) << (8 * i);
     }
     *reinterpret_cast<uint32_t*>(dst + k) = v;
   }

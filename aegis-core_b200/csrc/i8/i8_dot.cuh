@@ -34,12 +34,13 @@ struct DotArgs {
 
 inline constexpr int kDotThreads = 256, kDotWarps = kDotThreads / 32, kDotChannels = 4;
 
-// 16 codes at column k of a row whose pieces are 16-byte aligned; codes from column K on are zero.
+// 16 codes at column k (plain loads: the grid before this one may have written them while this one
+// was starting, which the read-only path must not see) of a row whose pieces are 16-byte aligned; codes from column K on are zero.
 __device__ __forceinline__ uint4 piece16(const int8_t* row, int k, int K) {
-  if (k + 16 <= K) return __ldg(reinterpret_cast<const uint4*>(row + k));
+  if (k + 16 <= K) return *reinterpret_cast<const uint4*>(row + k);
   uint32_t v[4] = {0, 0, 0, 0};
   for (int i = 0; k + i < K; ++i) {
-    const uint32_t b = uint8_t(__ldg(row + k + i));
+    const uint32_t b = uint8_t(row[k + i]);
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] |= (i >> 2) == j ? b << (8 * (i & 3)) : 0u;
   }
@@ -135,7 +136,7 @@ __global__ void __launch_bounds__(kDotThreads, 2) i8_dot_kernel(const __grid_con
     if (n >= a.N) continue;
     int s = 0;
     for (int p = 0; p < a.parts; ++p) s += sums[g * a.parts + p][c * MT + m];
-    const float sa = __ldg(a.a_scale + m), sw = __ldg(a.w_scale + n);
+    const float sa = a.a_scale[m], sw = a.w_scale[n];
     const float v = a.bias ? scaled(s, sa, sw, load_as_f32(a.bias, n, a.out)) : scaled(s, sa, sw);
     store_one(a.C, (long long)m * a.ldc + n, v, a.out);
   }

@@ -331,8 +331,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       const Unit u = umma::decode_unit_pair<kPairBN>(a, unit);
       const int row = u.m0 + row_in_tile;
       const bool live = row < a.M;
-      const float sa = live ? __ldg(p.a_scale + row) : 0.f;
-      const float sw = u.n0 + et < a.N ? __ldg(p.w_scale + u.n0 + et) : 0.f;
+      const float sa = live ? p.a_scale[row] : 0.f;
+      const float sw = u.n0 + et < a.N ? p.w_scale[u.n0 + et] : 0.f;
       float bias[kHalf / 32];
 #pragma unroll
       for (int c = 0; c < kHalf / 32; ++c) {

@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
     }
     const uint32_t t_row = tmem_base + (uint32_t(quarter * 32) << 16);
     const bool live = n < n_end;
-    const float sw = live ? __ldg(a.w_scale + n) : 0.f;
+    const float sw = live ? a.w_scale[n] : 0.f;
     const float b = live && a.bias ? load_as_f32(a.bias, n, a.out) : 0.f;
     constexpr int CH = NT < 32 ? NT : 32;
     for (int c = 0; c < mt && ok; c += CH) {
@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
 #pragma unroll
           for (int j = 0; j < CH; ++j) {
             if (c + j >= mt) break;
-            const float sa = __ldg(a.a_scale + m0 + c + j);
+            const float sa = a.a_scale[m0 + c + j];
             const float v = a.bias ? scaled(int(r[j]), sa, sw, b) : scaled(int(r[j]), sa, sw);
             store_one(a.C, (long long)(m0 + c + j) * a.ldc + n, v, a.out);
           }
@@ -269,13 +269,13 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
         sum.z += v.z;
         sum.w += v.w;
       }
-      const float sa = __ldg(a.a_scale + m0 + t);
+      const float sa = a.a_scale[m0 + t];
       const int acc[4] = {sum.x, sum.y, sum.z, sum.w};
       const int n = n0 + nl;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if (n + j < n_end) {
-          const float sw = __ldg(a.w_scale + n + j);
+          const float sw = a.w_scale[n + j];
           const float v = a.bias ? scaled(acc[j], sa, sw, load_as_f32(a.bias, n + j, a.out)) : scaled(acc[j], sa, sw);
           store_one(a.C, (long long)(m0 + t) * a.ldc + n + j, v, a.out);
         }
