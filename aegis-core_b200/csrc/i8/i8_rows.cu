@@ -166,7 +166,7 @@ struct Row {
   __device__ double t64(int c) const {
     if constexpr (MODE == kSilu) {
       const double g = double(Elem<T>::to_f32(x[c])), u = double(Elem<T>::to_f32(r[c]));
-      if (g == 0.0 || u == 0.0) return 0.0;
+      if ((g == 0.0 && fabs(u) <= kMost) || (u == 0.0 && fabs(g) <= kMost)) return 0.0;  // 0 times infinity is NaN
       return g / (1.0 + exp(-g)) * u;
     } else {
       return norm_input(c) * double(Elem<T>::to_f32(w[c]));

@@ -322,6 +322,26 @@ def zero_or_not_finite(ops, dtype, cols, rows):
     assert h.isinf().all() and s.isnan().all() and (q == 0).all()
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("rows,cols", [(7, 72), (7, 1001), (7, 40000), (3000, 64), (700, 12000)])
+def test_not_finite_next_to_zero(ops, dtype, rows, cols):
+    """NaN and infinity in one half do not vanish where the other half is 0."""
+    import torch
+    dt = getattr(torch, dtype)
+    g = gen(torch, rows + cols)
+    gate, up = (torch.randn(rows, cols, device="cuda", generator=g).to(dt) for _ in range(2))
+    nan, inf = float("nan"), float("inf")
+    for i, (a, b) in enumerate([(nan, 0), (inf, 0), (-inf, 0), (0, inf), (0, nan), (-0.0, -inf), (0, 0)]):
+        gate[i::7, (5 * i) % cols], up[i::7, (5 * i) % cols] = a, b
+    q, s = ops.silu_mul_i8(gate, up)
+    gd = gate.double()
+    t = gd / (1 + torch.exp(-gd)) * up.double()
+    bad = t.isnan().any(dim=1)
+    assert bad.sum() == rows - rows // 7
+    assert torch.equal(s.isnan(), bad) and (q[bad] == 0).all()
+    check_codes(torch, q[~bad], t[~bad])
+
+
 @pytest.mark.parametrize("cols", [100, 4096, 40000])
 @pytest.mark.parametrize("size", [1e30, 1e19, 1e-15, 1e-22, 1e-30, 1e-36])
 def test_norm_of_very_large_and_small_rows(ops, cols, size):
