@@ -12,7 +12,7 @@
 // layout, its neighbours or the number of threads.
 //
 // Bound: memory for the norm, instruction issue and memory alike for silu (about
-// 25 instructions an element). The blocks that fit the GPU walk the rows, a thread
+// 20 instructions an element). The blocks that fit the GPU walk the rows, a thread
 // with up to 32 elements, so what a row costs besides its elements (reduction,
 // barrier) is spread over many. A thread copies its elements of the next row to
 // shared memory while it works on this one, and reads them itself, so the copies
@@ -53,18 +53,19 @@ struct RowArgs {
 
 // The error of z = t * (127 / m) in float, relative, with u = 2^-24.
 // Norm: t and m are exact; the factor and the product round once each: 2 u.
-// Silu, t = x / (1 + e) * y with e = 2^(-x log2 e): the power's argument is off by
-// 1.25 u |x| log2 e, the power by that and by 4 u; the sum u, the reciprocal 2 u,
-// two products 2 u; then the factor (m and the quotient rounded) 2 u and the last
-// product u: (1.25 |x| + 12) u, the first part for negative x alone.
-// The factor may come from the float maximum, off by (1.25 |x| + 9) u itself.
+// Silu, t = (x y) / (1 + e) with e = 2^(-x log2 e): x y is exact (two 16-bit factors);
+// the power's argument is off by 1.25 u |x| log2 e, the power by that and by 4 u; the
+// sum u, the reciprocal 2 u, the product u; then the factor (m and the quotient
+// rounded) 2 u and the last product u: (1.25 |x| + 11) u, the first part for negative
+// x alone. An x y above float's range makes the maximum infinite, one below it is off
+// by less than 2^-149, both fine (kTiny).
+// The factor may come from the float maximum, off by (1.25 |x| + 8) u itself.
 constexpr float kBorderNorm = 1.5e-7f;
 __device__ __forceinline__ float border_silu(float gate) { return fmaf(gate, 1.6e-7f, 1.4e-6f); }
 // How far below the float maximum the true one can lie, relative.
 __device__ __forceinline__ float near_max(float gate) { return 1.f - fmaf(gate, 1.5e-7f, 1.25e-6f); }
-// What that error bound needs: e far from overflow, and no product near the
-// end of float's range. Rows with other values are done in double.
-constexpr float kMostGate = 80.f, kMostUp = 1e15f;  // gates below 0 alone
+// What that error bound needs: e far from overflow. Rows with gates below -kMostGate are done in double.
+constexpr float kMostGate = 80.f;
 // Rows whose largest magnitude is below this are done in double: float's range ends near.
 constexpr float kTiny = 1e-20f;
 constexpr double kMost = 3.4028234663852886e38;  // the largest float
@@ -190,7 +191,7 @@ __device__ __forceinline__ float fast_reciprocal(float x) {
 __device__ __forceinline__ f32x2 silu_mul(f32x2 x, f32x2 y) {
   const float2 p = both(mul2(x, pair(-1.44269504f, -1.44269504f)));
   const float2 d = both(add2(pair(fast_exp2(p.x), fast_exp2(p.y)), pair(1.f, 1.f)));
-  return mul2(mul2(x, pair(fast_reciprocal(d.x), fast_reciprocal(d.y))), y);
+  return mul2(mul2(x, y), pair(fast_reciprocal(d.x), fast_reciprocal(d.y)));
 }
 
 template <class T> struct Pair;
@@ -203,20 +204,14 @@ struct Stats {
   using P = typename Pair<T>::type;
   float m = 0.f;   // max |t|
   f32x2 ss = 0;    // squares, of even and odd elements (norm)
-  uint32_t low = 0, high = 0;  // least gate, largest |up|, two at a time (silu)
-  __device__ void gate_up(uint32_t g, uint32_t u) {
+  uint32_t low = 0;  // least gate, two at a time (silu)
+  __device__ void least_gate(uint32_t g) {
     const P l = __hmin2(reinterpret_cast<const P&>(low), reinterpret_cast<const P&>(g));
-    const P h = __hmax2(reinterpret_cast<const P&>(high), __habs2(reinterpret_cast<const P&>(u)));
     low = reinterpret_cast<const uint32_t&>(l);
-    high = reinterpret_cast<const uint32_t&>(h);
   }
   __device__ float gate() const {  // magnitude of the least gate below 0
     const float2 f = Elem<T>::pair_to_f32(low);
     return -fminf(f.x, f.y);
-  }
-  __device__ float most_up() const {
-    const float2 f = Elem<T>::pair_to_f32(high);
-    return fmaxf(f.x, f.y);
   }
 };
 
@@ -231,7 +226,7 @@ __device__ __forceinline__ uint4 eval8(uint4 xv, uint4 yv, uint4 wv, f32x2 (&t)[
     const f32x2 f = widen<T>(x[i]);
     if constexpr (MODE == kSilu) {
       t[i] = silu_mul(f, widen<T>(y[i]));
-      st.gate_up(x[i], y[i]);
+      st.least_gate(x[i]);
     } else {
       t[i] = mul2(f, widen<T>(w[i]));
       st.ss = fma2(f, f, st.ss);
@@ -348,18 +343,18 @@ __device__ __forceinline__ float at(const f32x2 (&t)[4], int i) {
 
 // 8 codes n from t. An element nearer to a border than z's error, border |z|, has
 // to be taken again: with d the distance from z to n, d > 1/2 - border (|n| + 1/2).
-// `most` gathers a first test of all elements, (most > first_test(border)) if
-// there may be one: border (n^2 / 64 + 16) for border |n|, which is never less, and
-// d^2 for d, to spare the magnitudes.
-__device__ __forceinline__ uint2 quantise8(const f32x2 (&t)[4], float inv, float border, float& most) {
+// `most`, the largest d, is a first test: above first_test(border), where |n| is taken
+// as 127, there may be one among the 8. A test with n^2 in it (three more paired
+// products an element pair) passed fewer pieces and cost more.
+__device__ __forceinline__ uint2 quantise8(const f32x2 (&t)[4], float inv, float& most) {
   uint32_t code[8];
+  most = 0.f;
   const f32x2 inv2 = pair(inv, inv), up = pair(kRound, kRound);
-  const f32x2 minus = pair(-1.f, -1.f), b2 = pair(border / 64.f, border / 64.f);
+  const f32x2 minus = pair(-1.f, -1.f);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const f32x2 r = fma2(t[i], inv2, up), n = fma2(r, minus, up);  // -n
-    const f32x2 d = fma2(t[i], inv2, n);
-    most = max_abs_nan(most, both(fma2(mul2(n, b2), n, mul2(d, d))));
+    most = max_abs_nan(most, both(fma2(t[i], inv2, n)));
     const float2 f = both(r);
     code[2 * i] = __float_as_uint(f.x);
     code[2 * i + 1] = __float_as_uint(f.y);
@@ -368,7 +363,7 @@ __device__ __forceinline__ uint2 quantise8(const f32x2 (&t)[4], float inv, float
   const uint32_t d = __byte_perm(code[4], code[5], 0x0040), e = __byte_perm(code[6], code[7], 0x0040);
   return make_uint2(__byte_perm(a, b, 0x5410), __byte_perm(d, e, 0x5410));
 }
-__device__ __forceinline__ float first_test(float border) { return 0.2499998f - 16.5f * border; }
+__device__ __forceinline__ float first_test(float border) { return kNearBorder - 127.5f * border; }
 // A bit for each of the 8 elements that is nearer to a border than that.
 __device__ __forceinline__ uint32_t near_border(const f32x2 (&t)[4], float inv, float border) {
   uint32_t near = 0;
@@ -522,7 +517,7 @@ __global__ void __launch_bounds__(MOST, BLOCKS) i8_rows_kernel(const __grid_cons
       }
     }
     copy_commit();
-    const int in_double = MODE == kSilu && (st.gate() > kMostGate || (Elem<T>::kBf16 && st.most_up() > kMostUp));
+    const int in_double = MODE == kSilu && st.gate() > kMostGate;
     int any = in_double;
     const Found f = block_find<MODE>(st.m, both(st.ss).x + both(st.ss).y, st.gate(), &any, buf[par]);
     if (MODE == kSilu) behind.begin();
@@ -534,15 +529,15 @@ __global__ void __launch_bounds__(MOST, BLOCKS) i8_rows_kernel(const __grid_cons
     } else {
       const float inv = 127.f / f.m;
       const float border = MODE == kSilu ? border_silu(f.gate) : kBorderNorm;
-      float most = 0.f;
+      float most[kPieces];
+#pragma unroll
+      for (int v = 0; v < kPieces; ++v) {
+        most[v] = 0.f;
+        if (v < pieces) *reinterpret_cast<uint2*>(q + v * step) = quantise8(t[v], inv, most[v]);
+      }
 #pragma unroll
       for (int v = 0; v < kPieces; ++v)
-        if (v < pieces) *reinterpret_cast<uint2*>(q + v * step) = quantise8(t[v], inv, border, most);
-      if (most > first_test(border)) {
-#pragma unroll
-        for (int v = 0; v < kPieces; ++v)
-          if (v < pieces) near |= near_border(t[v], inv, border) << (8 * v);
-      }
+        if (most[v] > first_test(border)) near |= near_border(t[v], inv, border) << (8 * v);
       // The maximum in 64 bits is that of the elements which can be it.
       const float least = f.m * near_max(f.gate);
       if (MODE == kSilu && st.m >= least) {
@@ -602,7 +597,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) i8_row_kernel(const _
   } else {
     for (int v = 0; piece(v) < a.cols; ++v) load_eval8<T, MODE>(a, row, piece(v), t[0], st);
   }
-  int any = MODE == kSilu && (st.gate() > kMostGate || st.most_up() > kMostUp);
+  int any = MODE == kSilu && st.gate() > kMostGate;
   const Found f = block_find<MODE>(st.m, both(st.ss).x + both(st.ss).y, st.gate(), &any, buf);
   if (needs_double<MODE>(f, any)) {
     row_in_double<T, MODE>(a, ri, buf64);
@@ -614,17 +609,14 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) i8_row_kernel(const _
   const float least = f.m * near_max(f.gate);
   if (MODE != kSilu && tid == 0) a.scale[ri] = norm_scale(a, f);
   if constexpr (VPT > 0) {
-    float most = 0.f;
     uint32_t near = 0, can = 0;
 #pragma unroll
     for (int v = 0; v < VPT; ++v)
-      if (piece(v) < a.cols)
-        store_codes(q, piece(v), a.cols, a.vec_q, quantise8(t[v], inv, border, most));
-    if (most > first_test(border)) {
-#pragma unroll
-      for (int v = 0; v < VPT; ++v)
-        if (piece(v) < a.cols) near |= near_border(t[v], inv, border) << (8 * v);
-    }
+      if (piece(v) < a.cols) {
+        float most;
+        store_codes(q, piece(v), a.cols, a.vec_q, quantise8(t[v], inv, most));
+        if (most > first_test(border)) near |= near_border(t[v], inv, border) << (8 * v);
+      }
     if constexpr (MODE == kSilu) {
       if (st.m >= least) {
 #pragma unroll
@@ -666,8 +658,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) i8_row_kernel(const _
         Stats<T> unused;
         load_eval8<T, MODE>(a, row, c, t[0], unused);
       }
-      float most = 0.f;
-      store_codes(q, c, a.cols, a.vec_q, quantise8(t[0], inv, border, most));
+      float most;
+      store_codes(q, c, a.cols, a.vec_q, quantise8(t[0], inv, most));
       if (most > first_test(border))
         for (uint32_t b = near_border(t[0], inv, border); b; b &= b - 1) {
           const int k = c + __ffs(int(b)) - 1;
