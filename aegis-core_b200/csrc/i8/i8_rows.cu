@@ -22,6 +22,10 @@
 // meanwhile; they are set right after the next row's barrier. Few rows take more threads
 // with fewer elements each, for latency. Rows beyond 32768 elements, and rows
 // that do not start on 16-byte boundaries, are read directly.
+//
+// B200, cold L2: norm with the residual 8192 x 4096 42 us (5.6 TB/s of the bytes it
+// must move), without 22.7 (4.4); silu 4096 x 14336 55.7 (5.3), 8192 x 4864 42.5
+// (4.7), 16384 x 1024 20.8 (4.0: a row's fixed costs); a row of 4096 2.0.
 #include <algorithm>
 
 #include "../common.cuh"
@@ -482,7 +486,7 @@ __global__ void __launch_bounds__(MOST, BLOCKS) i8_rows_kernel(const __grid_cons
   const int rows_ahead = int(gridDim.x);
   const T* x = static_cast<const T*>(a.x) + (long long)blockIdx.x * a.ldx + c0;
   const T* r = MODE == kNorm ? nullptr : static_cast<const T*>(a.r) + (long long)blockIdx.x * a.ldr + c0;
-  const T* w = MODE == kSilu ? nullptr : static_cast<const T*>(a.w) + c0;
+  const T* w = MODE == kSilu ? nullptr : static_cast<const T*>(a.w) + (pieces ? c0 : 0);
   T* h = MODE == kAddNorm ? static_cast<T*>(a.h) + (long long)blockIdx.x * a.ldh + c0 : nullptr;
   int8_t* q = a.q + (long long)blockIdx.x * a.ldq + c0;
   const uint32_t mine = ptx::smem_addr(ahead) + uint32_t(tid) * 16u, source = blockDim.x * 16u;
@@ -490,9 +494,16 @@ __global__ void __launch_bounds__(MOST, BLOCKS) i8_rows_kernel(const __grid_cons
     copy16(mine + uint32_t(v * kSources) * source, x + v * step);
     if (MODE != kNorm) copy16(mine + uint32_t(v * kSources + 1) * source, r + v * step);
   };
+  // Pieces beyond the row's end are zeros throughout: they change no maximum or sum,
+  // so only copies and stores ask for them (branches around the rest cost a tenth).
 #pragma unroll
-  for (int v = 0; v < kPieces; ++v)
-    if (v < pieces) copy_piece(v);
+  for (int v = 0; v < kPieces; ++v) {
+    if (v < pieces) {
+      copy_piece(v);
+    } else {
+      for (int i = 0; i < kSources; ++i) ahead[(v * kSources + i) * int(blockDim.x) + tid] = make_uint4(0, 0, 0, 0);
+    }
+  }
   copy_commit();
 
   Behind<T> behind{a, top64};
@@ -507,14 +518,12 @@ __global__ void __launch_bounds__(MOST, BLOCKS) i8_rows_kernel(const __grid_cons
     copy_wait<0>();
 #pragma unroll
     for (int v = 0; v < kPieces; ++v) {
-      if (v < pieces) {
-        const uint4 xv = ptx::ld_shared_v4(mine + uint32_t(v * kSources) * source);
-        const uint4 yv = MODE == kNorm ? xv : ptx::ld_shared_v4(mine + uint32_t(v * kSources + 1) * source);
-        const uint4 hv = eval8<T, MODE>(xv, yv, MODE == kSilu ? xv : *reinterpret_cast<const uint4*>(w + v * step),
-                                        t[v], st);
-        if (MODE == kAddNorm) *reinterpret_cast<uint4*>(h + v * step) = hv;
-        if (more) copy_piece(v);
-      }
+      const uint4 xv = ptx::ld_shared_v4(mine + uint32_t(v * kSources) * source);
+      const uint4 yv = MODE == kNorm ? xv : ptx::ld_shared_v4(mine + uint32_t(v * kSources + 1) * source);
+      const uint4 hv = eval8<T, MODE>(
+          xv, yv, MODE == kSilu ? xv : *reinterpret_cast<const uint4*>(v < pieces ? w + v * step : w), t[v], st);
+      if (MODE == kAddNorm && v < pieces) *reinterpret_cast<uint4*>(h + v * step) = hv;
+      if (more && v < pieces) copy_piece(v);
     }
     copy_commit();
     const int in_double = MODE == kSilu && st.gate() > kMostGate;
@@ -532,8 +541,8 @@ __global__ void __launch_bounds__(MOST, BLOCKS) i8_rows_kernel(const __grid_cons
       float most[kPieces];
 #pragma unroll
       for (int v = 0; v < kPieces; ++v) {
-        most[v] = 0.f;
-        if (v < pieces) *reinterpret_cast<uint2*>(q + v * step) = quantise8(t[v], inv, most[v]);
+        const uint2 codes = quantise8(t[v], inv, most[v]);
+        if (v < pieces) *reinterpret_cast<uint2*>(q + v * step) = codes;
       }
 #pragma unroll
       for (int v = 0; v < kPieces; ++v)
@@ -543,9 +552,8 @@ __global__ void __launch_bounds__(MOST, BLOCKS) i8_rows_kernel(const __grid_cons
       if (MODE == kSilu && st.m >= least) {
 #pragma unroll
         for (int v = 0; v < kPieces; ++v)
-          if (v < pieces)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) can |= fabsf(at(t[v], i)) >= least ? 1u << (8 * v + i) : 0u;
+          for (int i = 0; i < 8; ++i) can |= fabsf(at(t[v], i)) >= least ? 1u << (8 * v + i) : 0u;
       }
       if (MODE != kSilu && tid == 0) a.scale[ri] = norm_scale(a, f);
     }
@@ -696,7 +704,7 @@ cudaError_t launch_rows(const RowArgs& a, int threads, int sms, cudaStream_t s) 
   static gpu::SmemOptIn optin;
   if (const cudaError_t e = optin.ensure(reinterpret_cast<const void*>(kern), size_t(kBytes) * MOST); e != cudaSuccess)
     return e;
-  const int fit = std::min(MOST * BLOCKS / threads, 16);
+  const int fit = std::min(MOST * BLOCKS / threads, 32);
   cudaLaunchAttribute pdl;
   const cudaLaunchConfig_t cfg = launch_config(unsigned(std::min(a.rows, sms * fit)), unsigned(threads),
                                                size_t(kBytes) * threads, s, &pdl);
@@ -705,8 +713,12 @@ cudaError_t launch_rows(const RowArgs& a, int threads, int sms, cudaStream_t s) 
 template <class T, int MODE>
 cudaError_t launch_rows(const RowArgs& a, int sms, cudaStream_t s) {
   const int threads = ceil_div(a.cols, 32 * 8 * kPieces) * 32;
-  if (threads <= 128) return launch_rows<T, MODE, 128, 6>(a, threads, sms, s);
-  if (threads <= 256) return launch_rows<T, MODE, 256, 3>(a, threads, sms, s);
+  // About 900 threads an SM at 72 registers, in blocks that fit the row (silu 16384 x
+  // 1024: 31 us with 16 blocks an SM at most, 24 with 28); the plain norm is level to 3%
+  // faster with fewer and 80 registers.
+  if (threads <= 128) return launch_rows<T, MODE, 128, MODE == kNorm ? 6 : 7>(a, threads, sms, s);
+  if (threads <= 224) return launch_rows<T, MODE, 224, 4>(a, threads, sms, s);
+  if (threads <= 288) return launch_rows<T, MODE, 288, 3>(a, threads, sms, s);
   if (threads <= 448) return launch_rows<T, MODE, 448, 2>(a, threads, sms, s);
   return launch_rows<T, MODE, 1024, 1>(a, threads, sms, s);
 }
