@@ -222,7 +222,7 @@ def check_norm(torch, q, s, h, w, eps):
 ROWS = [(1, 1), (1, 8), (3, 7), (5, 64), (2, 1000), (4, 1024), (3, 1025), (2, 2048), (5, 4096), (3, 4097), (2, 8192),
         (2, 14336), (2, 16385), (1, 28672), (3, 32768), (2, 32769), (2, 40001), (700, 896),
         # more rows than blocks
-        (9000, 100), (4800, 1031), (2500, 4096), (700, 4105), (700, 9000), (400, 17000)]
+        (9000, 100), (4800, 1031), (2500, 4096), (700, 3001), (700, 4105), (700, 9000), (400, 17000)]
 
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
