@@ -16,7 +16,11 @@
 // shared memory, the next 32 columns are on their way from TMEM while the present
 // ones are scaled and stored, 32 bytes a lane and store. With four warps, scales
 // from global memory and 16-byte stores it took 6.9 us of a 22.5 us launch
-// (256 x 14336 x 4096, B200).
+// (256 x 14336 x 4096, B200; 17.2 now).
+//
+// Bound: the tensor cores, and power. B200: 8192^3 344 us (3.2 POP/s, 94% of twice
+// the measured bf16 burst rate), 375 to 408 in a long run under the power cap; 2048 x 4096
+// x 4096 27.5 us (2.5), two waves of which the second is partly empty.
 #include "../umma2_kernel.cuh"
 #include "i8_common.cuh"
 
