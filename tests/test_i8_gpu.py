@@ -353,6 +353,29 @@ def test_norm_of_very_large_and_small_rows(ops, cols, size):
     check_norm(torch, q, s, x, w, 0.0)
 
 
+@pytest.mark.parametrize("rows,cols", [(8, 72), (8, 4097), (8, 40000), (2400, 1000), (700, 12000)])
+def test_silu_where_gate_times_up_leaves_the_range(ops, rows, cols):
+    """bf16: gate * up above float's range with a finite result, far below it, and subnormal gates."""
+    import torch
+    g = gen(torch, rows + cols)
+    gate, up = (torch.randn(rows, cols, device="cuda", generator=g) for _ in range(2))
+    gate[0::4, 3], up[0::4, 3] = -70.0, 2.0 ** 127
+    gate[1::4, cols - 1], up[1::4, cols - 1] = 3e38, 2.0  # the result itself is beyond it
+    gate[2::4] *= 1e-25
+    up[2::4] *= 1e-25
+    gate[2::4, 5], up[2::4, 5] = 1e-10, 1e-5
+    gate[3::4] *= 1e-39
+    up[3::4] *= 1e35
+    gate, up = gate.bfloat16(), up.bfloat16()
+    q, s = ops.silu_mul_i8(gate, up)
+    gd = gate.double()
+    t = gd / (1 + torch.exp(-gd)) * up.double()
+    beyond = torch.arange(rows, device="cuda") % 4 == 1
+    assert s[beyond].isnan().all() and (q[beyond] == 0).all()
+    m = check_codes(torch, q[~beyond], t[~beyond])
+    assert ((s[~beyond].double() - m / 127).abs() <= 2.0 ** -24 * m / 127 * (1 + 2.0 ** -20)).all()
+
+
 def test_silu_of_rows_below_the_range_of_exp(ops):
     import torch
     g = torch.full((2, 300), -95.0, device="cuda").bfloat16()
