@@ -73,7 +73,7 @@ constexpr float kMostGate = 80.f;
 // Rows whose largest magnitude is below this are done in double: float's range ends near.
 constexpr float kTiny = 1e-20f;
 constexpr double kMost = 3.4028234663852886e38;  // the largest float
-// Adding this rounds a float below 2^22 to a whole number (nearest, ties to
+// Adding it takes a float below 2^22 to the nearest whole number (ties to
 // even) and leaves that number's two's complement in the low bits, without
 // the conversion unit, which the exponential and the reciprocal need.
 constexpr float kRound = 12582912.f;  // 1.5 * 2^23
