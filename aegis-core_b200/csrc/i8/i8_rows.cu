@@ -23,9 +23,14 @@
 // with fewer elements each, for latency. Rows beyond 32768 elements, and rows
 // that do not start on 16-byte boundaries, are read directly.
 //
-// B200, cold L2: norm with the residual 8192 x 4096 42 us (5.6 TB/s of the bytes it
-// must move), without 22.7 (4.4); silu 4096 x 14336 55.7 (5.3), 8192 x 4864 42.5
-// (4.7), 16384 x 1024 20.8 (4.0: a row's fixed costs); a row of 4096 2.0.
+// The norm's squares are summed in 64 bits and its scale is rounded once, as silu's is:
+// a scale off by its last bit moves results of the product that takes it. Against
+// sums in float, the plain norm of 8192 x 4096 takes 24.4 us instead of 22.1 (a
+// conversion and a 64-bit operation an element), everything else within 4%.
+//
+// B200, cold L2: norm with the residual 8192 x 4096 42.7 us (5.5 TB/s of the bytes it
+// must move), without 24.4 (4.1); silu 4096 x 14336 55.7 (5.3), 8192 x 4864 42.5
+// (4.7), 16384 x 1024 20.8 (4.0: a row's fixed costs); a row of 4096 2.1.
 #include <algorithm>
 
 #include "../common.cuh"
@@ -51,6 +56,7 @@ struct RowArgs {
   int8_t* q;
   long long ldq;
   float* scale;
+  double per_col;  // 1 / cols
   int vec;    // every 16-bit row and the weight start on 16-byte boundaries
   int vec_q;  // every row of q starts on an 8-byte boundary
 };
@@ -207,7 +213,7 @@ template <class T>
 struct Stats {
   using P = typename Pair<T>::type;
   float m = 0.f;   // max |t|
-  f32x2 ss = 0;    // squares, of even and odd elements (norm)
+  double ss = 0.0; // squares (norm): exact products, summed in 64 bits so that the scale rounds once
   uint32_t low = 0;  // least gate, two at a time (silu)
   __device__ void least_gate(uint32_t g) {
     const P l = __hmin2(reinterpret_cast<const P&>(low), reinterpret_cast<const P&>(g));
@@ -233,7 +239,9 @@ __device__ __forceinline__ uint4 eval8(uint4 xv, uint4 yv, uint4 wv, f32x2 (&t)[
       st.least_gate(x[i]);
     } else {
       t[i] = mul2(f, widen<T>(w[i]));
-      st.ss = fma2(f, f, st.ss);
+      const float2 v = both(f);
+      st.ss = fma(double(v.x), double(v.x), st.ss);
+      st.ss = fma(double(v.y), double(v.y), st.ss);
     }
     st.m = max_abs_nan(st.m, both(t[i]));
   }
@@ -250,38 +258,35 @@ __device__ __forceinline__ void load_eval8(const RowArgs& a, const Row<T, MODE>&
   if constexpr (MODE == kAddNorm) store8(row.h, c, a.cols, a.vec, h);
 }
 
-// A block's results: max |t|, the sum of the squares, the magnitude of the least
-// gate. Magnitudes are compared as the bits of floats without a sign, where a NaN
-// is above infinity.
+// A block's results: max |t|, the magnitude of the least gate. Magnitudes are
+// compared as the bits of floats without a sign, where a NaN is above infinity.
+// The squares' sum is kept by warp: only the scale needs it (norm_scale).
 struct Found {
-  float m, ss, gate;
+  float m, gate;
+  double ss;
 };
 __device__ __forceinline__ float max_bits(float v) {
   return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
 }
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
 template <int MODE>
-__device__ __forceinline__ Found block_find(float m, float ss, float gate, int* any, Found* buf) {
+__device__ __forceinline__ Found block_find(float m, double ss, float gate, int* any, Found* buf) {
   const int W = int(blockDim.x) / 32;
   const int lane = int(threadIdx.x & 31);
   Found f;
   f.m = max_bits(fabsf(m));
   f.gate = MODE == kSilu ? max_bits(fabsf(gate)) : 0.f;
-  if (MODE != kSilu)
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  f.ss = ss;
+  f.ss = MODE != kSilu ? warp_sum(ss) : 0.0;
   if (lane == 0) buf[threadIdx.x >> 5] = f;
   if (MODE == kSilu) *any = __syncthreads_or(*any);
   else __syncthreads();
   if (W > 1) {
-    f = lane < W ? buf[lane] : Found{0.f, 0.f, 0.f};
-    f.m = max_bits(f.m);
-    if (MODE == kSilu) {
-      f.gate = max_bits(f.gate);
-    } else {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) f.ss += __shfl_xor_sync(0xffffffffu, f.ss, o);
-    }
+    f.m = max_bits(lane < W ? buf[lane].m : 0.f);
+    if (MODE == kSilu) f.gate = max_bits(lane < W ? buf[lane].gate : 0.f);
   }
   return f;
 }
@@ -389,15 +394,20 @@ __device__ __forceinline__ void copy_wait() {
 }
 
 // Whether a row has to be taken in double: `gates` (silu, any thread's), a largest
-// magnitude that is tiny or not finite, squares that left float's range.
+// magnitude that is tiny or not finite.
 template <int MODE>
 __device__ __forceinline__ bool needs_double(const Found& f, int gates) {
-  const bool m = !(f.m >= kTiny && f.m <= 3.4028235e38f);
-  return MODE == kSilu ? m || gates : m || !(f.ss < 1e37f) || f.ss < 1e-25f;
+  return !(f.m >= kTiny && f.m <= 3.4028235e38f) || (MODE == kSilu && gates);
 }
 
-__device__ __forceinline__ float norm_scale(const RowArgs& a, const Found& f) {
-  return f.m / (127.f * sqrtf(f.ss / float(a.cols) + a.eps));
+// The norm's scale, m / sqrt(mean h^2 + eps) / 127, in 64 bits and rounded once: the
+// first warp joins the warps' sums that block_find left in buf and stores it. After
+// the codes, since nothing else of the row waits for it.
+__device__ __forceinline__ void norm_scale(const RowArgs& a, int ri, float m, const Found* buf) {
+  if (threadIdx.x >= 32) return;
+  const int W = int(blockDim.x) / 32, lane = int(threadIdx.x);
+  const double ss = warp_sum(lane < W ? buf[lane].ss : 0.0);
+  if (lane == 0) a.scale[ri] = float(double(m) * (1.0 / 127.0) * rsqrt(fma(ss, a.per_col, double(a.eps))));
 }
 
 // What a silu row leaves to do until the next row's barrier.
@@ -528,7 +538,7 @@ __global__ void __launch_bounds__(MOST, BLOCKS) i8_rows_kernel(const __grid_cons
     copy_commit();
     const int in_double = MODE == kSilu && st.gate() > kMostGate;
     int any = in_double;
-    const Found f = block_find<MODE>(st.m, both(st.ss).x + both(st.ss).y, st.gate(), &any, buf[par]);
+    const Found f = block_find<MODE>(st.m, st.ss, st.gate(), &any, buf[par]);
     if (MODE == kSilu) behind.begin();
     const bool done = needs_double<MODE>(f, any);
     uint32_t near = 0, can = 0;
@@ -555,7 +565,7 @@ __global__ void __launch_bounds__(MOST, BLOCKS) i8_rows_kernel(const __grid_cons
 #pragma unroll
           for (int i = 0; i < 8; ++i) can |= fabsf(at(t[v], i)) >= least ? 1u << (8 * v + i) : 0u;
       }
-      if (MODE != kSilu && tid == 0) a.scale[ri] = norm_scale(a, f);
+      if (MODE != kSilu) norm_scale(a, ri, f.m, buf[par]);
     }
     if constexpr (MODE == kSilu) {
       for (; can; can &= can - 1) behind.candidate(ri, __ffs(int(can)) - 1);
@@ -606,7 +616,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) i8_row_kernel(const _
     for (int v = 0; piece(v) < a.cols; ++v) load_eval8<T, MODE>(a, row, piece(v), t[0], st);
   }
   int any = MODE == kSilu && st.gate() > kMostGate;
-  const Found f = block_find<MODE>(st.m, both(st.ss).x + both(st.ss).y, st.gate(), &any, buf);
+  const Found f = block_find<MODE>(st.m, st.ss, st.gate(), &any, buf);
   if (needs_double<MODE>(f, any)) {
     row_in_double<T, MODE>(a, ri, buf64);
     return;
@@ -615,7 +625,6 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) i8_row_kernel(const _
   const float inv = 127.f / f.m;
   const float border = MODE == kSilu ? border_silu(f.gate) : kBorderNorm;
   const float least = f.m * near_max(f.gate);
-  if (MODE != kSilu && tid == 0) a.scale[ri] = norm_scale(a, f);
   if constexpr (VPT > 0) {
     uint32_t near = 0, can = 0;
 #pragma unroll
@@ -640,6 +649,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) i8_row_kernel(const _
     } else if (near) {
       set_codes<T, MODE>(a, ri, near, f.m);
     }
+    if (MODE != kSilu) norm_scale(a, ri, f.m, buf);
   } else {
     double m64 = double(f.m);
     if constexpr (MODE == kSilu) {
@@ -674,6 +684,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) i8_row_kernel(const _
           if (k < a.cols) q[k] = int8_t(code64<T, MODE>(row, k, m64));
         }
     }
+    if (MODE != kSilu) norm_scale(a, ri, f.m, buf);
   }
 }
 
@@ -761,6 +772,7 @@ RowArgs make_args(const RowOp& o) {
   a.ldr = o.ldr;
   a.w = o.weight;
   a.eps = o.eps;
+  a.per_col = 1.0 / double(o.cols);
   a.h = o.h;
   a.ldh = o.ldh;
   a.q = static_cast<int8_t*>(o.q);
