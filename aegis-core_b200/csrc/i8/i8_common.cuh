@@ -39,9 +39,11 @@ __device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t a_desc, u
 // Makes this thread's shared-memory stores visible to the tensor core's reads.
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// Barrier of the cluster's threads that only keeps its CTAs in step: no CTA leaves
-// before the others have read its shared memory. cluster_sync's release would also
-// wait for this thread's stores to C to be visible (0.7 us).
+// Barrier of the cluster's threads that orders no memory operation: a thread that has
+// passed it knows only that every other one has come to it. Loads whose values have been
+// used before, and remote arrivals that were waited for where they go, are over then;
+// a remote store or arrival that nobody has waited for is not. cluster_sync's release
+// covers those, and waits for this thread's stores to C to be visible too (0.7 us).
 __device__ __forceinline__ void cluster_step() {
   asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }

@@ -23,6 +23,7 @@
 // x 4096 27.5 us (2.5), two waves of which the second is partly empty.
 #include "../umma2_kernel.cuh"
 #include "i8_common.cuh"
+#include "i8_phases.h"
 
 namespace aegis::i8 {
 
@@ -266,6 +267,12 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                        : umma::sched_take(sched, seq, true, &unit, kStatusTimeoutProducer);
       }
       owner.drain(sched);
+      // The leader: every reader has given its slots back, the peer's arrivals for them have landed.
+      if (rank == 0 && a.steal && ok)
+        for (int i = 0; i < umma::kSchedDepth; ++i)
+          if (!ptx::mbar_wait_teardown(sched.empty_bar(i), slot_read(owner.seq, i, umma::kSchedDepth), a.wait_limit_ns) &&
+              a.status)
+            atomicOr(a.status, kStatusTimeoutDrain);
       for (int s = 0; s < STAGES; ++s)
         if (filled & (1u << s)) {
           const uint32_t par = (fill_parity >> s) & 1u;
@@ -279,18 +286,19 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     // ------------------------------------------------ MMA issuer (leader only)
     if (rank == 0) {
       constexpr uint32_t idesc = idesc_i8(umma::BM_PAIR, kPairBN);
-      int stage = 0, acc = 0;
-      uint32_t phase = 0, acc_phase = 0;
+      int stage = 0;
+      uint32_t phase = 0;
+      AccumulatorTurn turn;
       bool ok = true;
       if (lane == 0) {
         int seq = 0;
         for (long long unit = first_unit; ok && unit >= 0;) {
           const Unit u = umma::decode_unit_pair<kPairBN>(a, unit);
-          ok = ptx::mbar_wait_bounded(tempty_bar(acc), acc_phase ^ 1u, abort_flag, a.status, kStatusTimeoutMma,
+          ok = ptx::mbar_wait_bounded(tempty_bar(turn.acc), turn.read(turn.acc), abort_flag, a.status, kStatusTimeoutMma,
                                       a.wait_limit_ns);
           if (!ok) break;
           ptx::tc_fence_after();
-          const uint32_t d_tmem = tmem_base + uint32_t(acc * kPairBN);
+          const uint32_t d_tmem = tmem_base + uint32_t(turn.acc * kPairBN);
           for (int i = 0; i < u.nkb; ++i) {
             ok = ptx::mbar_wait_bounded(full_bar(stage), phase, abort_flag, a.status, kStatusTimeoutMma,
                                         a.wait_limit_ns);
@@ -311,12 +319,16 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             }
           }
           if (!ok) break;
-          ptx::umma_commit_pair(tfull_bar(acc), 0x3);
-          acc ^= 1;
-          if (acc == 0) acc_phase ^= 1u;
+          ptx::umma_commit_pair(tfull_bar(turn.acc), 0x3);
+          turn.next();
           if (!a.steal) break;
           ok = umma::sched_take(sched, seq, false, &unit, kStatusTimeoutMma);
         }
+        // Both accumulators have been read for the last time: the peer's arrivals that say so have landed.
+        if (ok)
+          for (int acc = 0; acc < 2; ++acc)
+            if (!ptx::mbar_wait_teardown(tempty_bar(acc), turn.read(acc), a.wait_limit_ns) && a.status)
+              atomicOr(a.status, kStatusTimeoutDrain);
       }
       __syncwarp();
     }
@@ -327,8 +339,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     const int et = int(threadIdx.x) - 64;                            // 0..255: the column whose scale it fetches
     const int row_in_tile = 128 * int(rank) + quarter * 32 + lane;
     const uint32_t scales = sbase + L::SCALE_OFF;
-    int acc = 0;
-    uint32_t acc_phase = 0;
+    AccumulatorTurn turn;
     bool ok = true;
     int seq = 0;
     for (long long unit = first_unit; ok && unit >= 0;) {
@@ -347,13 +358,13 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       asm volatile("st.shared.f32 [%0], %1;" ::"r"(scales + 4u * uint32_t(et)), "f"(sw) : "memory");
       ptx::named_barrier(1, 32 * kPairEpilogueWarps);
       if (lane == 0)
-        ok = ptx::mbar_wait_bounded(tfull_bar(acc), acc_phase, abort_flag, a.status, kStatusTimeoutEpilogue,
+        ok = ptx::mbar_wait_bounded(tfull_bar(turn.acc), turn.full(), abort_flag, a.status, kStatusTimeoutEpilogue,
                                     a.wait_limit_ns);
       // One answer for all eight warps: a warp that left alone would strand the others at the barriers.
       ok = named_all(2, 32 * kPairEpilogueWarps, __shfl_sync(0xffffffffu, ok, 0));
       if (!ok) break;
       ptx::tc_fence_after();
-      const uint32_t t_row = tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(acc * kPairBN + first);
+      const uint32_t t_row = tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(turn.acc * kPairBN + first);
       RowWriter<T> out(static_cast<T*>(a.C) + (live ? row : 0) * a.ldc + u.n0 + first);
       uint32_t r[2][32];
       ptx::tmem_ld_32x32b_x32(t_row, r[0]);
@@ -365,7 +376,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         } else {
           ptx::tc_fence_before();
           __syncwarp();
-          if (lane == 0) arrive_relaxed(ptx::map_to_rank(tempty_bar(acc), 0));  // the accumulator is read
+          if (lane == 0) arrive_relaxed(ptx::map_to_rank(tempty_bar(turn.acc), 0));  // the accumulator is read
         }
         const int col = u.n0 + first + 32 * c;
         if (col >= a.N) continue;
@@ -382,8 +393,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         }
       }
       if (live) out.finish();
-      acc ^= 1;
-      if (acc == 0) acc_phase ^= 1u;
+      turn.next();
       if (!a.steal) break;
       long long next = -1;
       if (lane == 0) ok = umma::sched_take(sched, seq, rank != 0, &next, kStatusTimeoutEpilogue);
@@ -401,7 +411,12 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   }
   __syncwarp();
   ptx::tc_fence_before();
-  cluster_step();  // neither CTA leaves while its peer may still touch its memory
+  // Neither CTA leaves while its peer may still touch its memory. What is sent to the
+  // peer's CTA has been waited for there: the leader's slots and accumulators above, the
+  // peer's copies on the leader's full barriers, the leader's commits and slots by the
+  // peer's roles. After a wait that ran out that is not known, so the barrier itself orders it.
+  if (*abort_flag) ptx::cluster_sync();
+  else cluster_step();
   ptx::tc_fence_after();
   if (warp == 1) ptx::tmem_dealloc_pair(tmem_base, L::TMEM_COLS);
 }
