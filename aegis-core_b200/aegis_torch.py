@@ -29,8 +29,9 @@ into CUDA graphs after one call on the device, and have fake implementations.
 Rows may be strided (stride(-1) == 1, rows that do not overlap); other stride
 patterns are copied first. The int8 results have rows padded to 16 bytes
 (stride(0) is a multiple of 16), which is what the product reads fastest.
-They have no backward pass: an input that requires a gradient is refused
-while gradients are recorded.
+They have no derivatives: an input that requires a gradient while gradients
+are recorded, or that carries a forward tangent, is refused, under torch.func's
+transforms too.
 """
 from __future__ import annotations
 
@@ -115,14 +116,6 @@ _defs.define("mlp_i8(Tensor x, Tensor residual, Tensor norm_weight, float eps, T
              "Tensor w_down, Tensor s_down) -> (Tensor, Tensor)")
 
 
-def _no_grad(name: str, *tensors) -> None:
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise RuntimeError(f"aegis::{name} has no backward pass: call it under torch.no_grad() or detach "
-                                   "its inputs")
-
-
 def _same_device(name: str, first: torch.Tensor, *others) -> None:
     d = first.device
     for t in others:
@@ -159,7 +152,6 @@ def _check_matmul_i8(a, w, a_scale, w_scale, bias, out_dtype):
         if bias.dim() != 1 or bias.shape[0] != w.shape[0]:
             raise ValueError(f"aegis::matmul_i8: bias must have shape ({w.shape[0]},), not {tuple(bias.shape)}")
     _same_device(name, a, w, a_scale, w_scale, bias)
-    _no_grad(name, a_scale, w_scale, bias)
     return out_dtype
 
 
@@ -198,7 +190,6 @@ def _check_norm(name, x, residual, weight, eps):
     if not 0.0 <= eps <= 3.4e38:
         raise ValueError(f"aegis::{name}: eps must be a finite number, 0 or more")
     _same_device(name, x, residual, weight)
-    _no_grad(name, x, residual, weight)
 
 
 def _rmsnorm_i8_meta(x, weight, eps):
@@ -214,7 +205,6 @@ def _add_rmsnorm_i8_meta(x, residual, weight, eps):
 def _check_silu_mul(gate, up):
     _check_rows("silu_mul_i8", gate, up, "up")
     _same_device("silu_mul_i8", gate, up)
-    _no_grad("silu_mul_i8", gate, up)
 
 
 def _silu_mul_i8_meta(gate, up):
@@ -239,7 +229,6 @@ def _check_mlp(x, residual, norm_weight, eps, w_gate_up, s_gate_up, w_down, s_do
     _f32_vector(name, "s_gate_up", s_gate_up, 2 * F)
     _f32_vector(name, "s_down", s_down, K)
     _same_device(name, x, w_gate_up, s_gate_up, w_down, s_down)
-    _no_grad(name, s_gate_up, s_down)
 
 
 def _mlp_i8_meta(x, residual, norm_weight, eps, w_gate_up, s_gate_up, w_down, s_down):

@@ -5,6 +5,7 @@
 // loads this library. Arguments are checked here as there.
 #include <ATen/core/Tensor.h>
 #include <ATen/core/grad_mode.h>
+#include <ATen/core/stack.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_strided.h>
 #include <c10/cuda/CUDAStream.h>
@@ -32,11 +33,22 @@ int code_of(at::ScalarType t) {
 
 void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 
-void no_grad(const char* name, std::initializer_list<const Tensor*> ts) {
-  if (!at::GradMode::is_enabled()) return;
-  for (const Tensor* t : ts)
-    TORCH_CHECK(!t->defined() || !t->requires_grad(), "aegis::", name,
-                " has no backward pass: call it under torch.no_grad() or detach its inputs");
+// The Autograd kernel of every operator here: there are no derivatives, and an input
+// that asks for one must not pass as a constant. It stands at this key, and not in the
+// kernels below it, because torch.func's transforms show their gradients and tangents
+// only here.
+void refuse_derivatives(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch::jit::Stack* stack) {
+  const bool reverse = at::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+  if (reverse || forward)
+    for (const c10::IValue& v : torch::jit::last(*stack, op.schema().arguments().size())) {
+      if (!v.isTensor() || !v.toTensor().defined()) continue;
+      const Tensor& t = v.toTensor();
+      TORCH_CHECK(!reverse || !t.requires_grad(), op.schema().name(),
+                  " has no backward pass: call it under torch.no_grad() or detach its inputs");
+      TORCH_CHECK(!forward || !t._fw_grad(0).defined(), op.schema().name(),
+                  " has no forward derivative: an input has a tangent");
+    }
+  op.redispatchBoxed(keys & c10::after_autograd_keyset, stack);
 }
 
 void same_device(const char* name, const Tensor& first, std::initializer_list<const Tensor*> ts) {
@@ -107,7 +119,6 @@ Tensor matmul_i8(const Tensor& a, const Tensor& w, const Tensor& a_scale, const 
                       bias.sizes());
   }
   same_device(name, a, {&w, &a_scale, &w_scale, &bias});
-  no_grad(name, {&a_scale, &w_scale, &bias});
   Tensor out = at::empty({M, N}, a.options().dtype(dt));
   if (M == 0 || N == 0) return out;
   const Rows ra(a), rw(w);
@@ -145,7 +156,6 @@ void check_norm(const char* name, const Tensor& x, const Tensor& residual, const
                     x.size(1), ",), not ", weight.sizes());
   TORCH_CHECK_VALUE(eps >= 0.0 && eps <= 3.4e38, "aegis::", name, ": eps must be a finite number, 0 or more");
   same_device(name, x, {&residual, &weight});
-  no_grad(name, {&x, &residual, &weight});
 }
 
 // (q, scale) for the rows of x: int8 rows 16 bytes aligned, one float a row.
@@ -188,7 +198,6 @@ std::tuple<Tensor, Tensor> silu_mul_i8(const Tensor& gate, const Tensor& up) {
   const char* name = "silu_mul_i8";
   check_rows(name, gate, up, "up");
   same_device(name, gate, {&up});
-  no_grad(name, {&gate, &up});
   auto [q, scale] = empty_codes(gate);
   if (gate.size(0)) {
     const Rows g(gate), u(up);
@@ -218,7 +227,6 @@ std::tuple<Tensor, Tensor> mlp_i8(const Tensor& x, const Tensor& residual, const
   f32_vector(name, "s_gate_up", s_gate_up, 2 * F);
   f32_vector(name, "s_down", s_down, K);
   same_device(name, x, {&w_gate_up, &s_gate_up, &w_down, &s_down});
-  no_grad(name, {&s_gate_up, &s_down});
   Tensor y = at::empty({M, K}, x.options()), h = at::empty({M, K}, x.options());
   if (M) {
     const Rows rx(x), rr(residual), w1(w_gate_up), w2(w_down);
@@ -242,4 +250,9 @@ TORCH_LIBRARY_IMPL(aegis, CUDA, m) {
   m.impl("add_rmsnorm_i8", &add_rmsnorm_i8);
   m.impl("silu_mul_i8", &silu_mul_i8);
   m.impl("mlp_i8", &mlp_i8);
+}
+
+TORCH_LIBRARY_IMPL(aegis, Autograd, m) {
+  for (const char* name : {"matmul_i8", "rmsnorm_i8", "add_rmsnorm_i8", "silu_mul_i8", "mlp_i8"})
+    m.impl(name, torch::CppFunction::makeFromBoxedFunction<&refuse_derivatives>());
 }

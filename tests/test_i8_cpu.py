@@ -233,3 +233,46 @@ def test_gradients_may_be_off():
     x = meta(4, 8).requires_grad_()
     with torch.no_grad():
         assert ops.rmsnorm_i8(x, meta(8), 1e-5)[0].shape == (4, 8)
+
+
+def calls_with(x):
+    """Every operator with `x` ([8, 16] bfloat16, meta) or its rows among the inputs."""
+    a, w, f = meta(8, 16, dtype=I8), meta(4, 16, dtype=I8), lambda n: meta(n, dtype=F32)
+    return [
+        lambda: ops.rmsnorm_i8(x, meta(16), 1e-5)[1],
+        lambda: ops.rmsnorm_i8(meta(3, 16), x[0], 1e-5)[1],
+        lambda: ops.add_rmsnorm_i8(meta(8, 16), x, meta(16), 1e-5)[2],
+        lambda: ops.silu_mul_i8(meta(8, 16), x)[1],
+        lambda: ops.matmul_i8(a, w, x[:, 0].float(), f(4)),
+        lambda: ops.matmul_i8(a, w, f(8), x[0, :4].float()),
+        lambda: ops.matmul_i8(a, w, f(8), f(4), x[0, :4]),
+        lambda: ops.mlp_i8(x, meta(8, 16), meta(16), 1e-5, meta(40, 16, dtype=I8), f(40), meta(16, 20, dtype=I8), f(16))[0],
+        lambda: ops.mlp_i8(meta(8, 16), meta(8, 16), meta(16), 1e-5, meta(40, 16, dtype=I8), f(40),
+                           meta(16, 20, dtype=I8), x[0].float())[0],
+    ]
+
+
+@pytest.mark.parametrize("which", range(9))
+def test_derivatives_of_every_kind_are_refused(which):
+    import torch.autograd.forward_ad as fwad
+    x = meta(8, 16)
+    with pytest.raises(RuntimeError, match="no backward"):
+        calls_with(x.clone().requires_grad_())[which]()
+    with fwad.dual_level():
+        with pytest.raises(RuntimeError, match="tangent"):
+            calls_with(fwad.make_dual(x, meta(8, 16)))[which]()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="tangent"):  # it does not switch tangents off
+            calls_with(fwad.make_dual(x, meta(8, 16)))[which]()
+        calls_with(x)[which]()
+
+    def total(v):
+        return calls_with(v)[which]().float().sum()
+    for transform in (torch.func.grad(total), torch.func.jacfwd(total), torch.func.jacrev(total),
+                      lambda v: torch.func.jvp(total, (v,), (v,))):
+        with pytest.raises(RuntimeError, match="no backward|tangent"):
+            transform(x)
+    with torch.no_grad():
+        calls_with(x.clone().requires_grad_())[which]()
+    with torch.inference_mode():
+        calls_with(meta(8, 16))[which]()
+    assert torch.func.vmap(lambda v: ops.silu_mul_i8(v, v)[1], in_dims=1)(meta(8, 3, 16)).shape == (3, 8)
