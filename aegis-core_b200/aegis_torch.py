@@ -241,8 +241,28 @@ for _name, _meta in (("matmul_i8", _matmul_i8_meta), ("rmsnorm_i8", _rmsnorm_i8_
                      ("mlp_i8", _mlp_i8_meta)):
     _defs.impl(_name, _meta, "Meta")
 
-# The CUDA implementations (csrc/i8/torch_ops.cpp) call libaegis_i8.so.
+# The CUDA implementations (csrc/i8/torch_ops.cpp) call libaegis_i8.so. Without these
+# libraries matmul is there all the same, and calls of the 8-bit operators raise.
 _TORCH_LIB = os.path.join(ac.HERE, "build", "libaegis_torch_i8.so")
-if not os.path.exists(_TORCH_LIB):
-    raise FileNotFoundError(f"{_TORCH_LIB} is not built: run `make -C aegis-core_b200` (or __graft_entry__.build())")
-torch.ops.load_library(_TORCH_LIB)
+
+
+def _unavailable(name: str, why: str):
+    def call(*args, **kwargs):
+        raise RuntimeError(f"aegis::{name}: {why}")
+    return call
+
+
+def _load_i8() -> bool:
+    why = f"{_TORCH_LIB} is not built: run `make -C aegis-core_b200 all torch` (or __graft_entry__.build())"
+    if os.path.exists(_TORCH_LIB):
+        try:
+            torch.ops.load_library(_TORCH_LIB)
+            return True
+        except OSError as e:  # libaegis_i8.so is missing, or another torch's library
+            why = f"{_TORCH_LIB} cannot be loaded: {e}"
+    for name in ("matmul_i8", "rmsnorm_i8", "add_rmsnorm_i8", "silu_mul_i8", "mlp_i8"):
+        _defs.impl(name, _unavailable(name, why), "CUDA")
+    return False
+
+
+I8_LOADED = _load_i8()
