@@ -72,7 +72,10 @@ int on_device(int device, const char* fn, F&& body, bool launch = true) {
     cudaGetLastError();
     return fail(AEGIS_ERR_NO_DEVICE, fn, "no such CUDA device");
   }
-  const cudaError_t e = body();
+  // The device's status word is made by its first launch, whichever operator's: the next one may be captured.
+  unsigned* status = nullptr;
+  cudaError_t e = launch ? aegis::status::word(&status) : cudaSuccess;
+  if (e == cudaSuccess) e = body();
   return e == cudaSuccess ? AEGIS_OK : fail_cuda(fn, e, launch);
 }
 

@@ -16,8 +16,9 @@
  *     context: two threads may call at once.
  *   - Nothing is allocated or kept from one call for the next, except, on the
  *     first call of a device, 16 bytes for the watchdog's status and the
- *     kernels' shared-memory limits: make that call before a stream capture.
- *     All calls may be captured into CUDA graphs after that.
+ *     kernels' shared-memory limits: make that call, of any operator, before a
+ *     stream capture (a no-op does not count). All calls may be captured into
+ *     CUDA graphs after that.
  *   - Operands are device pointers of that device. Leading dimensions count
  *     elements, and every alignment is accepted. Rows of codes whose addresses
  *     are multiples of 16 bytes are read as they are, others from an aligned
