@@ -65,13 +65,30 @@ __device__ __forceinline__ float load_as_f32(const void* p, long long i, Out t) 
   return Elem<__half>::to_f32(static_cast<const __half*>(p)[i]);
 }
 
-// acc * a_scale * w_scale + bias. The conversion of acc to float rounds sums
+// A token's scale, s * f: f is 1, but for scales from 2^97 on, with which a sum of up
+// to 2^31 would leave float's range before the channel's scale brings it back. Those are
+// taken 2^64 smaller (the product with any channel's scale is then below the range only
+// where it is 0) and the result 2^64 larger, both exact. Small scales need nothing: a
+// whole number times one of float's smallest is not rounded.
+struct TokenScale {
+  float s, f;
+};
+__device__ __forceinline__ TokenScale token_scale(float sa) {
+  const bool large = fabsf(sa) >= 0x1p97f;
+  return {large ? sa * 0x1p-64f : sa, large ? 0x1p64f : 1.f};
+}
+
+// acc * a_scale * w_scale (+ bias). The conversion of acc to float rounds sums
 // above 2^24 (relative 2^-24); each step is one float rounding, written as
 // separate intrinsics so every kernel gives the same bits.
-__device__ __forceinline__ float scaled(int acc, float sa, float sw, float bias) {
-  return __fadd_rn(__fmul_rn(__fmul_rn(float(acc), sa), sw), bias);
+__device__ __forceinline__ float scaled(int acc, float s, float sw) { return __fmul_rn(__fmul_rn(float(acc), s), sw); }
+__device__ __forceinline__ float scaled(int acc, const TokenScale& sa, float sw) {
+  const float v = scaled(acc, sa.s, sw);
+  return sa.f == 1.f ? v : __fmul_rn(v, sa.f);
 }
-__device__ __forceinline__ float scaled(int acc, float sa, float sw) { return __fmul_rn(__fmul_rn(float(acc), sa), sw); }
+__device__ __forceinline__ float scaled(int acc, const TokenScale& sa, float sw, float bias) {
+  return __fadd_rn(scaled(acc, sa, sw), bias);
+}
 
 __device__ __forceinline__ void store_one(void* c, long long i, float v, Out t) {
   if (t == Out::F32) static_cast<float*>(c)[i] = v;

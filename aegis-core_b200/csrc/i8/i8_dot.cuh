@@ -137,7 +137,8 @@ __global__ void __launch_bounds__(kDotThreads, 2) i8_dot_kernel(const __grid_con
     if (n >= a.N) continue;
     int s = 0;
     for (int p = 0; p < a.parts; ++p) s += sums[g * a.parts + p][c * MT + m];
-    const float sa = a.a_scale[m], sw = a.w_scale[n];
+    const TokenScale sa = token_scale(a.a_scale[m]);
+    const float sw = a.w_scale[n];
     const float v = a.bias ? scaled(s, sa, sw, load_as_f32(a.bias, n, a.out)) : scaled(s, sa, sw);
     store_one(a.C, (long long)m * a.ldc + n, v, a.out);
   }

@@ -74,15 +74,19 @@ __device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
 
 // 32 channels of one token: scaled by sa and the scales at `scales` (shared memory),
 // plus the bias (one value a lane, for its channel).
-__device__ __forceinline__ void scale_chunk(const PairArgs& a, float sa, uint32_t scales, float bias,
+__device__ __forceinline__ void scale_chunk(const PairArgs& a, const TokenScale& sa, uint32_t scales, float bias,
                                             const uint32_t (&r)[32], float (&v)[32]) {
 #pragma unroll
   for (int i = 0; i < 32; i += 4) {
     const uint4 w = ptx::ld_shared_v4(scales + 4 * i);
-    v[i] = scaled(int(r[i]), sa, __uint_as_float(w.x));
-    v[i + 1] = scaled(int(r[i + 1]), sa, __uint_as_float(w.y));
-    v[i + 2] = scaled(int(r[i + 2]), sa, __uint_as_float(w.z));
-    v[i + 3] = scaled(int(r[i + 3]), sa, __uint_as_float(w.w));
+    v[i] = scaled(int(r[i]), sa.s, __uint_as_float(w.x));
+    v[i + 1] = scaled(int(r[i + 1]), sa.s, __uint_as_float(w.y));
+    v[i + 2] = scaled(int(r[i + 2]), sa.s, __uint_as_float(w.z));
+    v[i + 3] = scaled(int(r[i + 3]), sa.s, __uint_as_float(w.w));
+  }
+  if (sa.f != 1.f) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __fmul_rn(v[i], sa.f);
   }
   if (a.bias) {
 #pragma unroll
@@ -346,7 +350,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       const Unit u = umma::decode_unit_pair<kPairBN>(a, unit);
       const int row = u.m0 + row_in_tile;
       const bool live = row < a.M;
-      const float sa = live ? p.a_scale[row] : 0.f;
+      const TokenScale sa = token_scale(live ? p.a_scale[row] : 0.f);
       const float sw = u.n0 + et < a.N ? p.w_scale[u.n0 + et] : 0.f;
       float bias[kHalf / 32];
 #pragma unroll

@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
 #pragma unroll
           for (int j = 0; j < CH; ++j) {
             if (c + j >= mt) break;
-            const float sa = a.a_scale[m0 + c + j];
+            const TokenScale sa = token_scale(a.a_scale[m0 + c + j]);
             const float v = a.bias ? scaled(int(r[j]), sa, sw, b) : scaled(int(r[j]), sa, sw);
             store_one(a.C, (long long)(m0 + c + j) * a.ldc + n, v, a.out);
           }
@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
         sum.z += v.z;
         sum.w += v.w;
       }
-      const float sa = a.a_scale[m0 + t];
+      const TokenScale sa = token_scale(a.a_scale[m0 + t]);
       const int acc[4] = {sum.x, sum.y, sum.z, sum.w};
       const int n = n0 + nl;
 #pragma unroll

@@ -56,7 +56,8 @@ AEGIS_API int aegis_i8_synchronize(int device, void* stream);
  * layout of torch.nn.Linear.weight), row stride ldw >= K. a_scale: M floats,
  * w_scale: N floats. bias: N values of out_dtype, or NULL. C: M x N of
  * out_dtype (AEGIS_DTYPE_F16, _BF16 or _F32), row stride ldc >= N.
- * The sum is exact (int32); it is converted to float, scaled, the bias added
+ * The sum is exact (int32); it is converted to float, scaled (scales may come
+ * near the ends of float's range: no step between leaves it), the bias added
  * in float, and rounded once. K = 0: the sum is 0. M or N = 0: no-op.
  * K > AEGIS_I8_MAX_K, negative sizes, too-small strides, null operands:
  * AEGIS_ERR_INVALID_ARGUMENT. Results do not depend on the alignment of the
