@@ -39,8 +39,9 @@ struct GemmPlan {
 };
 GemmPlan plan_gemm(int M, int N, int K, int sms);
 
-// Whether TMA can address the rows: 16-byte aligned base, stride a multiple of 16.
-bool tma_rows(const void* p, long long ld);
+// Whether TMA can address the rows: 16-byte aligned base, and a stride that is a
+// multiple of 16 where there is more than one.
+bool tma_rows(const void* p, long long ld, int rows);
 
 // Columns of a copy whose rows TMA can address: whole blocks of 128.
 constexpr size_t aligned_cols(int K) { return (size_t(K) + 127) / 128 * 128; }

@@ -151,8 +151,8 @@ struct MlpSpace {
     gu = take(size_t(M) * size_t(ldgu) * 2);
     q2 = take(size_t(M) * size_t(ld2));
     s2 = take(size_t(M) * 4);
-    copy1 = !aegis::i8::tma_rows(w_gate_up, ld_gate_up);
-    copy2 = !aegis::i8::tma_rows(w_down, ld_down);
+    copy1 = !aegis::i8::tma_rows(w_gate_up, ld_gate_up, 2 * F);
+    copy2 = !aegis::i8::tma_rows(w_down, ld_down, K);
     w1 = take(copy1 ? 2 * size_t(F) * aegis::i8::aligned_cols(K) : 0);
     w2 = take(copy2 ? size_t(K) * aegis::i8::aligned_cols(F) : 0);
     bytes = at;

@@ -11,7 +11,9 @@
 
 namespace aegis::i8 {
 
-bool tma_rows(const void* p, long long ld) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 16 == 0; }
+bool tma_rows(const void* p, long long ld, int rows) {
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (rows <= 1 || ld % 16 == 0);
+}
 
 namespace {
 
@@ -235,8 +237,8 @@ cudaError_t align(const void* src, long long ld, int rows, int K, void* dst, cud
 
 GemmSpace gemm_space(const void* A, long long lda, const void* W, long long ldw, int M, int N, int K) {
   GemmSpace sp;
-  sp.w = K > 0 && !tma_rows(W, ldw) ? size_t(N) * aligned_cols(K) : 0;
-  sp.a = K > 0 && !tma_rows(A, lda) ? size_t(M) * aligned_cols(K) : 0;
+  sp.w = K > 0 && !tma_rows(W, ldw, N) ? size_t(N) * aligned_cols(K) : 0;
+  sp.a = K > 0 && !tma_rows(A, lda, M) ? size_t(M) * aligned_cols(K) : 0;
   return sp;
 }
 
@@ -248,7 +250,9 @@ cudaError_t gemm(const Gemm& g, cudaStream_t s) {
   if (const cudaError_t e = status::word(&status); e != cudaSuccess) return e;
   const GemmPlan p = plan_gemm(g.M, g.N, g.K, d->sms);
   // Copies of rows that TMA cannot address: the weights' first, then the tokens'.
-  Rows ra{g.A, g.lda, g.K}, rw{g.W, g.ldw, g.K};
+  // A single row's stride means nothing: a tensor map gets one that it can hold.
+  const long long one = (long long)aligned_cols(std::max(g.K, 1));
+  Rows ra{g.A, g.M > 1 ? g.lda : one, g.K}, rw{g.W, g.N > 1 ? g.ldw : one, g.K};
   const GemmSpace space = gemm_space(g.A, g.lda, g.W, g.ldw, g.M, g.N, g.K);
   char* ws = static_cast<char*>(g.workspace);
   if (space.w || space.a)

@@ -66,7 +66,8 @@ AEGIS_API int aegis_i8_gemm(int device, void* stream, int out_dtype, int M, int 
                             const void* W, int64_t ldw, const float* a_scale, const float* w_scale,
                             const void* bias, void* C, int64_t ldc, void* workspace, size_t workspace_bytes);
 /* Bytes of workspace that call needs: 0 where the addresses of all rows of A and
- * W are multiples of 16 bytes. Makes no CUDA call. */
+ * W are multiples of 16 bytes (of a single row: its address alone). Makes no
+ * CUDA call. */
 AEGIS_API int aegis_i8_gemm_workspace(int M, int N, int K, const void* A, int64_t lda, const void* W, int64_t ldw,
                                       size_t* bytes);
 

@@ -276,3 +276,13 @@ def test_derivatives_of_every_kind_are_refused(which):
     with torch.inference_mode():
         calls_with(meta(8, 16))[which]()
     assert torch.func.vmap(lambda v: ops.silu_mul_i8(v, v)[1], in_dims=1)(meta(8, 3, 16)).shape == (3, 8)
+
+
+def test_a_single_row_has_no_stride():
+    """Its address alone says whether it needs a copy, whatever the stride given with it."""
+    assert i8.gemm_workspace(1, 8, 33, P, 33, P, 48) == 0
+    assert i8.gemm_workspace(4, 1, 33, P, 48, P, 33) == 0
+    assert i8.gemm_workspace(1, 1, 33, P, 33, P, 35) == 0
+    assert i8.gemm_workspace(1, 8, 33, P + 1, 48, P, 48) == 128 and i8.gemm_workspace(4, 1, 33, P, 48, P + 8, 48) == 128
+    assert i8.gemm_workspace(2, 8, 33, P, 33, P, 48) == 2 * 128
+    assert i8.mlp_workspace(3, 1, 65, P, 16, P, 65) == i8.mlp_workspace(3, 1, 65, P, 16, P, 80)
