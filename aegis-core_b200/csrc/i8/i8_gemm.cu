@@ -78,7 +78,7 @@ GemmPlan plan_gemm(int M, int N, int K, int sms) {
     p.grid = 2 * pair_tiles;
   }
   for (const StreamVariant& v : kStream) {
-    if (v.tokens > 16 && v.tokens >= 2 * M) break;  // a smaller tile holds them all
+    if (v.tokens > 16 && v.tokens / 2 >= M) break;  // a smaller tile holds them all
     const long long token_tiles = ceil_div(M, v.tokens), slots = (long long)sms * v.ctas_per_sm;
     const int steps = ceil_div(kb, v.group);
     for (int S = 1; S <= 8 && S <= std::max(1, steps); S *= 2) {

@@ -286,3 +286,16 @@ def test_a_single_row_has_no_stride():
     assert i8.gemm_workspace(1, 8, 33, P + 1, 48, P, 48) == 128 and i8.gemm_workspace(4, 1, 33, P, 48, P + 8, 48) == 128
     assert i8.gemm_workspace(2, 8, 33, P, 33, P, 48) == 2 * 128
     assert i8.mlp_workspace(3, 1, 65, P, 16, P, 65) == i8.mlp_workspace(3, 1, 65, P, 16, P, 80)
+
+
+@pytest.mark.parametrize("N,K", [(64, 0), (64, 128), (1, 4096), (4096, 16)])
+def test_plans_of_the_largest_sizes(N, K):
+    """As many tokens as the calls accept are planned as their neighbours are."""
+    most = 2 ** 31 - 2 ** 20
+    for M in (2 ** 30 - 1, 2 ** 30, most):
+        p, q = i8.gemm_plan(M, N, K), i8.gemm_plan(2 ** 29, N, K)
+        assert (p["kernel"], p["tile_m"], p["tile_n"], p["splits"]) == (q["kernel"], q["tile_m"], q["tile_n"], q["splits"])
+        assert p["tiles"] == -(-M // p["tile_m"]) * -(-N // p["tile_n"])
+    for M in (1, 300):
+        p = i8.gemm_plan(M, most, K)
+        assert p["tiles"] == -(-M // p["tile_m"]) * -(-most // p["tile_n"])
