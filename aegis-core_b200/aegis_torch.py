@@ -123,6 +123,16 @@ def _same_device(name: str, first: torch.Tensor, *others) -> None:
             raise ValueError(f"aegis::{name}: operands on different devices ({d} and {t.device})")
 
 
+_MAX_SIZE = 2 ** 31 - 2 ** 20  # the C calls' limit
+
+
+def _sizes_fit(name: str, *tensors) -> None:
+    for t in tensors:
+        for n in t.shape:
+            if n > _MAX_SIZE:
+                raise ValueError(f"aegis::{name}: a size above 2^31 - 2^20")
+
+
 def _f32_vector(name: str, what: str, t: torch.Tensor, n) -> None:
     if t.dtype != torch.float32:
         raise TypeError(f"aegis::{name}: {what} must be float32, not {t.dtype}")
@@ -140,6 +150,7 @@ def _check_matmul_i8(a, w, a_scale, w_scale, bias, out_dtype):
         raise ValueError(f"aegis::matmul_i8: a [M, K] and w [N, K] have different K ({tuple(a.shape)}, {tuple(w.shape)})")
     if a.shape[1] > i8.MAX_K:
         raise ValueError(f"aegis::matmul_i8: K above {i8.MAX_K}: the int32 sum could overflow")
+    _sizes_fit(name, a, w)
     _f32_vector(name, "a_scale", a_scale, a.shape[0])
     _f32_vector(name, "w_scale", w_scale, w.shape[0])
     if out_dtype is None:
@@ -174,6 +185,7 @@ def _check_rows(name, x, y, what):
         raise TypeError(f"aegis::{name}: operands must be float16 or bfloat16, not {x.dtype}")
     if x.shape[1] == 0:
         raise ValueError(f"aegis::{name}: rows of no elements have no scale")
+    _sizes_fit(name, x)
     if y is not None:
         if y.dtype != x.dtype:
             raise TypeError(f"aegis::{name}: {what} must have x's type, {x.dtype}, not {y.dtype}")

@@ -299,3 +299,20 @@ def test_plans_of_the_largest_sizes(N, K):
     for M in (1, 300):
         p = i8.gemm_plan(M, most, K)
         assert p["tiles"] == -(-M // p["tile_m"]) * -(-most // p["tile_n"])
+
+
+@pytest.mark.parametrize("n,refused", [(2 ** 31 - 2 ** 20, False), (2 ** 31 - 2 ** 20 + 1, True), (2 ** 32 + 4, True)])
+def test_sizes_that_the_gpu_refuses_are_refused_as_fakes(n, refused):
+    calls = [lambda: ops.matmul_i8(meta(n, 16, dtype=I8), meta(4, 16, dtype=I8), meta(n, dtype=F32), meta(4, dtype=F32)),
+             lambda: ops.matmul_i8(meta(4, 16, dtype=I8), meta(n, 16, dtype=I8), meta(4, dtype=F32), meta(n, dtype=F32)),
+             lambda: ops.rmsnorm_i8(meta(n, 8), meta(8), 1e-5), lambda: ops.rmsnorm_i8(meta(2, n), meta(n), 1e-5),
+             lambda: ops.add_rmsnorm_i8(meta(n, 8), meta(n, 8), meta(8), 1e-5),
+             lambda: ops.silu_mul_i8(meta(n, 8), meta(n, 8)),
+             lambda: ops.mlp_i8(meta(n, 48), meta(n, 48), meta(48), 1e-5, meta(40, 48, dtype=I8), meta(40, dtype=F32),
+                                meta(48, 20, dtype=I8), meta(48, dtype=F32))]
+    for call in calls:
+        if refused:
+            with pytest.raises(ValueError, match="size"):
+                call()
+        else:
+            call()
