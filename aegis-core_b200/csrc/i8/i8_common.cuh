@@ -36,9 +36,6 @@ __device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t a_desc, u
       : "memory");
 }
 
-// Makes this thread's shared-memory stores visible to the tensor core's reads.
-__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-
 // Barrier of the cluster's threads that orders no memory operation: a thread that has
 // passed it knows only that every other one has come to it. Loads whose values have been
 // used before, and remote arrivals that were waited for where they go, are over then;

@@ -35,8 +35,9 @@ struct DotArgs {
 
 inline constexpr int kDotThreads = 256, kDotWarps = kDotThreads / 32, kDotChannels = 4;
 
-// 16 codes at column k (plain loads: the grid before this one may have written them while this one
-// was starting, which the read-only path must not see) of a row whose pieces are 16-byte aligned; codes from column K on are zero.
+// 16 codes at column k of a row whose pieces are 16-byte aligned; codes from column K on
+// are zero. Plain loads: the grid before this one may have written the codes while this
+// one was starting, and the read-only path could miss that.
 __device__ __forceinline__ uint4 piece16(const int8_t* row, int k, int K) {
   if (k + 16 <= K) return *reinterpret_cast<const uint4*>(row + k);
   uint32_t v[4] = {0, 0, 0, 0};
