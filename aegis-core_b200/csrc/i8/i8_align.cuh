@@ -8,8 +8,8 @@
 // such pieces of a row are on their way at once. The product's own loads from
 // unaligned rows, shifted on their way into the shared-memory ring, reached 1.4 TB/s
 // for few tokens and a tenth of the tensor rate for many. B200, us, that and this
-// copy with the product: 1 x 14336 x 4095 43, 31; 256 x 14336 x 4095 120, 45;
-// 2048 x 4096 x 4095 220, 42.
+// copy with the product: 1 x 14336 x 4095 43, 32; 256 x 14336 x 4095 120, 37;
+// 2048 x 4096 x 4095 220, 37.
 #include "i8_common.cuh"
 
 namespace aegis::i8 {

@@ -8,7 +8,7 @@
 //
 // Bound: the weight stream. A token's codes come out of L1 after the first
 // warp's read; 4 channels share each read. dp4a runs at 64 lanes a clock and
-// SM, which at 8 tokens and the weights' rate (23 B a clock and SM) is three
+// SM; 8 tokens at the weights' rate from DRAM (23 B a clock and SM) would keep it three
 // quarters busy: more tokens belong on the tensor cores. B200, cold L2: 1 x 4096 x 4096
 // 6.0 us (2.8 TB/s; launch to launch 1.4 and the first loads' 1.2 are half of it).
 //

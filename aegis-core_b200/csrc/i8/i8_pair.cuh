@@ -16,11 +16,15 @@
 // shared memory, the next 32 columns are on their way from TMEM while the present
 // ones are scaled and stored, 32 bytes a lane and store. With four warps, scales
 // from global memory and 16-byte stores it took 6.9 us of a 22.5 us launch
-// (256 x 14336 x 4096, B200; 17.2 now).
+// (256 x 14336 x 4096, B200; 17.4 now).
 //
-// Bound: the tensor cores, and power. B200: 8192^3 344 us (3.2 POP/s, 94% of twice
-// the measured bf16 burst rate), 375 to 408 in a long run under the power cap; 2048 x 4096
-// x 4096 27.5 us (2.5), two waves of which the second is partly empty.
+// The leader's last waits, for its peer's arrivals, cost 1 us at the end where tiles come
+// from the schedule: a slot is given back behind the peer's stores.
+//
+// Bound: the tensor cores, and power. B200: 8192^3 357 us (3.1 POP/s, 91% of twice
+// the measured bf16 burst rate), 361 to 408 in a long run under the power cap; 2048 x 4096
+// x 4096 28.6 us (2.4), two waves of which the second is partly empty; 512 x 4096 x
+// 14336 38.5 us, 64 of 148 SMs.
 #include "../umma2_kernel.cuh"
 #include "i8_common.cuh"
 #include "i8_phases.h"
@@ -104,7 +108,7 @@ __device__ __forceinline__ T to_out(float v) {
 // 16-byte boundary (every other row of an odd N, say) the values are shifted to
 // the boundaries in registers, the last 16 bytes of a chunk waiting for the next
 // one: single 2-byte stores, 32 rows of them an instruction, took four times the
-// whole product's time (1000 x 14331 x 4096: 190 us, the aligned N 48).
+// whole product's time (1000 x 14331 x 4096: 190 us; now 60, the aligned N 50).
 template <class T>
 struct RowWriter {
   static constexpr int kWords = 32 * int(sizeof(T)) / 4;  // a chunk's

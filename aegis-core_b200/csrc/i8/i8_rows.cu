@@ -11,8 +11,9 @@
 // codes are computed again in double. Codes therefore do not depend on a row's
 // layout, its neighbours or the number of threads.
 //
-// Bound: memory for the norm, instruction issue and memory alike for silu (about
-// 20 instructions an element). The blocks that fit the GPU walk the rows, a thread
+// Bound: memory, and instruction issue not far behind: 24 instructions an element and
+// 64% of the issue slots for the norm with its residual, 19 and 62% without, 20 and 60%
+// for silu, whose exponential and reciprocal take half of their unit's time too. The blocks that fit the GPU walk the rows, a thread
 // with up to 32 elements, so what a row costs besides its elements (reduction,
 // barrier) is spread over many. A thread copies its elements of the next row to
 // shared memory while it works on this one, and reads them itself, so the copies

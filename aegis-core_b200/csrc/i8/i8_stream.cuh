@@ -18,8 +18,8 @@
 //
 // Bound: the weights from DRAM, and about 5 us a launch in which DRAM is not busy
 // (the end of the last grid to this one's wait 1.4, first copies 1.2, joining and the
-// tail). B200, cold L2, us: 16 x 4096 x 4096 7.4 (2.3 TB/s), 16 x 14336 x 4096 14.1
-// (4.2), 16 x 28672 x 4096 21.3 (5.5). Two CTAs an SM fill its shared memory; smaller
+// tail). B200, cold L2, us: 16 x 4096 x 4096 7.4 (2.3 TB/s), 16 x 14336 x 4096 14.2
+// (4.2), 16 x 28672 x 4096 21.5 (5.5). Two CTAs an SM fill its shared memory; smaller
 // rings, with which the next launch's CTAs fit beside these, were 2 to 14% slower.
 //
 // Every wait is bounded; on expiry the CTA records a status bit, its roles
