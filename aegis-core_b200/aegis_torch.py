@@ -27,8 +27,9 @@ The 8-bit operators (include/aegis_i8.h has their definitions; sm_100 only):
 They run on torch's current stream of their operands' device, may be captured
 into CUDA graphs after one call on the device, and have fake implementations.
 Rows may be strided (stride(-1) == 1, rows that do not overlap); other stride
-patterns are copied first. eps is taken in 32 bits. The int8 results have rows padded to 16 bytes
-(stride(0) is a multiple of 16), which is what the product reads fastest.
+patterns are copied first. The int8 results have rows padded to 16 bytes
+(stride(0) is a multiple of 16), which is what the product reads fastest. eps
+is taken in 32 bits.
 They have no derivatives: an input that requires a gradient while gradients
 are recorded, or that carries a forward tangent, is refused, under torch.func's
 transforms too.
